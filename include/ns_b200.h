@@ -50,6 +50,9 @@ enum {
 /* Activation of a gate. */
 enum { NS_ACT_SILU = 0, NS_ACT_SIGMOID = 1, NS_ACT_GELU = 2, NS_ACT_RELU = 3 };
 
+/* Which columns of a head rotary positions turn together: 2 p and 2 p + 1, or p and p + rot_dims / 2. */
+enum { NS_ROTARY_PAIRS = 0, NS_ROTARY_HALVES = 1 };
+
 /* How a Linear layer is divided among tensor-parallel ranks. */
 enum { NS_SPLIT_NONE = 0, NS_SPLIT_COLUMN = 1, NS_SPLIT_ROW = 2 };
 
@@ -284,6 +287,20 @@ NS_API int ns_f32_penalize_rows(ns_device_t dev, uint64_t logits, uint64_t work,
 /* [261] HistoryPush (history_push_f32, PtxKernels.Decoding.cs:435-447): history[r, length[0] % capacity] = ids[r]. */
 NS_API int ns_f32_history_push(ns_device_t dev, uint64_t ids, uint64_t history, uint64_t length, int rows, int capacity);
 
+/* The next token of every row from a random number that the caller gives, every row with a temperature, top-k, top-p and min-p of its own
+ * (requests of a batch; ns_f32_sample_rows has one setting for all rows and draws its own numbers).  Row r reads vocab logits at logits + r * row_stride
+ * (elements; dtype NS_F32 or NS_BF16) and keeps, with weights w_j = e^((x_j - max x) / temperature[r]),
+ *   the first top_k[r] tokens by (x descending, index ascending)        (0 or less: all),
+ *   of those the shortest beginning whose weights reach top_p[r] times the sum of theirs, one token at least        (1 or more: all),
+ *   of those the ones with w >= min_p[r]        (0 or less: all; more than 1 counts as 1).
+ * ids[r] (int32) is the first token in the vocabulary's order at which the running sum of kept weights exceeds u[r] times their sum, u[r] in [0, 1);
+ * probs[r] (float; probs may be 0) its weight over that sum.  A temperature that is not above 0 takes the first maximum.  NaN counts as -infinity; where all
+ * are, ids[r] = -1 and probs[r] = 0.  temperature, top_p, min_p float [rows], top_k int32 [rows]: each may be 0, which leaves that step out (temperature: 1).
+ * Weights are computed in 64 bits and summed exactly in units of 2^-44 (smaller ones are never drawn), so a row's token does not depend on the other
+ * rows or their number.  vocab at most 408 000 floats or 816 000 bf16. */
+NS_API int ns_sample_tokens(ns_device_t dev, uint64_t logits, int dtype, int64_t row_stride, int rows, int vocab, uint64_t temperature, uint64_t top_k,
+                            uint64_t top_p, uint64_t min_p, uint64_t u, uint64_t ids, uint64_t probs);
+
 /* ------------------------------------------------------------------------------------------------
  * Key/value cache and attention.  Replaces KeyValueCache + Tensor.WriteKeyValues (Layers/Decoding.cs:14-35,
  * Tensor.Decoding.cs:62-66 -> kv_write_f32, PtxKernels.Decoding.cs:130-143) and the three-kernel attention of
@@ -334,6 +351,25 @@ NS_API int ns_attention_decode(ns_device_t dev, ns_kv_cache_t cache, uint64_t q,
 NS_API int ns_attention_decode_quant(ns_device_t dev, ns_kv_cache_t cache, uint64_t q, int64_t q_stride, uint64_t o, int64_t o_stride,
                                      uint64_t page_table, int max_pages, uint64_t pos_dev, int batch, int steps, float scale, uint64_t q_out,
                                      uint64_t q_scale);
+
+/* Rotary positions of query and key heads.  The first rot_dims columns of each head are turned, pair by pair (layout NS_ROTARY_*):
+ *   (a, b) -> amplitude * (a cos t - b sin t, a sin t + b cos t),  t = pos[row] * freq[pair]  (inverse != 0: -t; with the same amplitude
+ * that is the gradient), and the others copied.  Head h of row r is at x[r * x_ld + h * x_head], pitches in elements; y likewise, either x itself
+ * with x's pitches, or a matrix that does not overlap it.  x and y are both NS_F32 or NS_BF16; pos int32 [rows], rows of a negative position are
+ * left as they are in y; freq float [rot_dims / 2].  t is computed in 64 bits, the rest in 32.  rot_dims even, dim <= 4096. */
+NS_API int ns_rotary(ns_device_t dev, uint64_t x, int dtype, int64_t x_ld, int64_t x_head, uint64_t pos, uint64_t freq, float amplitude, int layout,
+                     int inverse, int64_t rows, int heads, int dim, int rot_dims, uint64_t y, int64_t y_ld, int64_t y_head);
+
+/* ns_kv_append for query heads in groups, sequences at positions of their own, and with rotary positions on the way.  Row b * steps + i of the source (a product as its row
+ * kernel reads it, described at the operators of recurrent decoders below) holds `heads` query heads from column q_col on, the cache's number of
+ * key heads from k_col, of value heads from v_col.  Token i of sequence b is at position pos[b] + i of its pages (pos int32 [batch], page_table int32
+ * [batch, max_pages]) and its queries and keys are turned as ns_rotary does for position offset[0] + pos[b] + i (offset one int32 word, may be 0: the length of a prefix
+ * that lies in other pages).  q: bf16 rows of q_ld elements (0: keys and values alone).  lens int32 [batch] (may be 0): tokens i >= lens[b] are
+ * padding; nothing of theirs is written.  A position or page outside the table or the pool: queries only, status 500 (NS_ERR_KERNEL).  No two
+ * tokens of a call may share a place in the pool. */
+NS_API int ns_kv_append_rotary(ns_device_t dev, ns_kv_cache_t cache, uint64_t src, int splits, int src_dtype, int src_ld, int q_col, int k_col, int v_col,
+                               int heads, uint64_t freq, float amplitude, int layout, int rot_dims, uint64_t offset, uint64_t pos, uint64_t lens,
+                               uint64_t page_table, int max_pages, int batch, int steps, uint64_t q, int64_t q_ld);
 
 /* Attention over a whole sequence (MultiHeadAttention.ForwardCore, Layers/Attention.cs:46-91) without the
  * [T, T] score tensor: o[b, h, i, :] = softmax_j((q[b,h,i,:] . k[b,h,j,:]) * scale + mask) . v[b,h,j,:], mask = -inf

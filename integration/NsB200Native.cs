@@ -291,6 +291,9 @@ internal static unsafe partial class NsB200Native
     public static partial int ns_f32_history_push(nint dev, ulong ids, ulong history, ulong length, int rows, int capacity);
 
     [LibraryImport(Library)]
+    public static partial int ns_sample_tokens(nint dev, ulong logits, int dtype, long row_stride, int rows, int vocab, ulong temperature, ulong top_k, ulong top_p, ulong min_p, ulong u, ulong ids, ulong probs);
+
+    [LibraryImport(Library)]
     public static partial int ns_kv_cache_create(nint dev, int num_pages, int page_size, int heads, int head_dim, out nint cache);
 
     [LibraryImport(Library)]
@@ -313,6 +316,12 @@ internal static unsafe partial class NsB200Native
 
     [LibraryImport(Library)]
     public static partial int ns_attention_decode_quant(nint dev, nint cache, ulong q, long q_stride, ulong o, long o_stride, ulong page_table, int max_pages, ulong pos_dev, int batch, int steps, float scale, ulong q_out, ulong q_scale);
+
+    [LibraryImport(Library)]
+    public static partial int ns_rotary(nint dev, ulong x, int dtype, long x_ld, long x_head, ulong pos, ulong freq, float amplitude, int layout, int inverse, long rows, int heads, int dim, int rot_dims, ulong y, long y_ld, long y_head);
+
+    [LibraryImport(Library)]
+    public static partial int ns_kv_append_rotary(nint dev, nint cache, ulong src, int splits, int src_dtype, int src_ld, int q_col, int k_col, int v_col, int heads, ulong freq, float amplitude, int layout, int rot_dims, ulong offset, ulong pos, ulong lens, ulong page_table, int max_pages, int batch, int steps, ulong q, long q_ld);
 
     [LibraryImport(Library)]
     public static partial int ns_attention_prefill(nint dev, ulong q, ulong k, ulong v, ulong o, int batch, int heads, int seq, int head_dim, long* q_strides, long* k_strides, long* v_strides, long* o_strides, float scale, int causal);

@@ -15,7 +15,7 @@
 #include <math.h>
 #include <string.h>
 
-#include "ns_common.cuh"
+#include "ns_cache.cuh"
 
 struct NsKvCache {
     int ordinal;
@@ -611,12 +611,6 @@ extern "C" int ns_kv_append(ns_device_t h, ns_kv_cache_t ch, uint64_t k, uint64_
     return NS_OK;
 }
 
-// The pools and geometry of a cache, for kernels in other files that write to it (ns_step_fused.cu).
-struct NsKvCacheView {
-    uint16_t* k_pool;
-    uint16_t* v_pool;
-    int page_size, heads, head_dim, num_pages;
-};
 int ns_kv_cache_view(ns_kv_cache_t ch, NsKvCacheView* out)
 {
     NsKvCache* c = reinterpret_cast<NsKvCache*>(ch);

@@ -15,15 +15,9 @@
 // results are bit-identical to the unfused sequence.
 #include <math.h>
 
+#include "ns_cache.cuh"
 #include "ns_gemm.cuh"
 #include "ns_rows.cuh"
-
-struct NsKvCacheView {
-    uint16_t* k_pool;
-    uint16_t* v_pool;
-    int page_size, heads, head_dim, num_pages;
-};
-int ns_kv_cache_view(ns_kv_cache_t cache, NsKvCacheView* out);   // ns_attention_decode.cu
 
 namespace {
 

@@ -15,6 +15,7 @@ LIB_PATH = os.path.join(_HERE, "libns_b200.so")
 NS_F32, NS_BF16, NS_I8, NS_I32 = 0, 1, 2, 3
 EPI_NONE, EPI_BIAS, EPI_BIAS_GELU, EPI_BIAS_RESIDUAL = 0, 1, 2, 3
 ACT_SILU, ACT_SIGMOID, ACT_GELU, ACT_RELU = 0, 1, 2, 3
+ROTARY_PAIRS, ROTARY_HALVES = 0, 1
 SPLIT_NONE, SPLIT_COLUMN, SPLIT_ROW = 0, 1, 2
 
 u64, i64, i32, u32, f32, vp, cp = C.c_uint64, C.c_int64, C.c_int, C.c_uint32, C.c_float, C.c_void_p, C.c_char_p
@@ -68,6 +69,7 @@ SIGNATURES = {
     "ns_convert": [vp, u64, i32, u64, i32, i64],
     "ns_fill_normal": [vp, u64, i32, i64, u32, f32, f32],
     "ns_fill_ids": [vp, u64, i64, u32, u32],
+    "ns_sample_tokens": [vp, u64, i32, i64, i32, i32, u64, u64, u64, u64, u64, u64, u64],
     "ns_kv_cache_create": [vp, i32, i32, i32, i32, P(vp)],
     "ns_kv_cache_create_in": [vp, i32, i32, i32, i32, u64, u64, P(vp)],
     "ns_kv_cache_destroy": [vp],
@@ -76,6 +78,8 @@ SIGNATURES = {
     "ns_kv_append": [vp, vp, u64, u64, i64, u64, i32, u64, i32, i32],
     "ns_attention_decode": [vp, vp, u64, i64, u64, i64, u64, i32, u64, i32, i32, f32],
     "ns_attention_prefill": [vp, u64, u64, u64, u64, i32, i32, i32, i32, P(i64), P(i64), P(i64), P(i64), f32, i32],
+    "ns_rotary": [vp, u64, i32, i64, i64, u64, u64, f32, i32, i32, i64, i32, i32, i32, u64, i64, i64],
+    "ns_kv_append_rotary": [vp, vp, u64, i32, i32, i32, i32, i32, i32, i32, u64, f32, i32, i32, u64, u64, u64, u64, i32, i32, i32, u64, i64],
     "ns_linear_create": [vp, i32, i32, i32, P(f32), P(f32), i32, i32, i32, i32, P(vp)],
     "ns_linear_destroy": [vp],
     "ns_linear_info": [vp, P(i32), P(i32), P(i32), P(u64), P(u64), P(u64)],
