@@ -352,6 +352,17 @@ NS_API int ns_attention_decode_quant(ns_device_t dev, ns_kv_cache_t cache, uint6
                                      uint64_t page_table, int max_pages, uint64_t pos_dev, int batch, int steps, float scale, uint64_t q_out,
                                      uint64_t q_scale);
 
+/* ns_attention_decode for a batch whose sequences share a prefix: o[b, i, h, :] = softmax_j(scale * q[b, i, h, :] . K_j) . V_j over the first prefix_len[0] positions
+ * of prefix_table (int32 [prefix_pages], the same for every sequence) and over the positions j <= pos[b] + i of the sequence's own pages
+ * (page_table int32 [batch, max_pages], pos int32 [batch]).  The prefix is read once for all sequences.  `heads` query heads, a multiple of the cache's: query
+ * head h reads key/value head h / (heads / the cache's heads).  q element (b, i, h, d) at q[(b * steps + i) * q_stride + h * head_dim + d], o likewise with
+ * o_stride.  lens int32 [batch] (may be 0): rows i >= lens[b] are padding and stay as they are in o.  Either part may be missing (prefix_pages 0 or max_pages 0, with its
+ * addresses 0); positions outside a table do not count, a row that sees none is zero.  A table entry that names no page of the pool: its positions are left out and status 520
+ * is reported (NS_ERR_KERNEL).  prefix_len, pos and the tables are device memory, read when the kernels run.  Uses the device object's scratch block. */
+NS_API int ns_attention_shared(ns_device_t dev, ns_kv_cache_t cache, uint64_t q, int64_t q_stride, uint64_t o, int64_t o_stride, int heads, uint64_t prefix_table,
+                               int prefix_pages, uint64_t prefix_len, uint64_t page_table, int max_pages, uint64_t pos, uint64_t lens, int batch, int steps,
+                               float scale);
+
 /* Rotary positions of query and key heads.  The first rot_dims columns of each head are turned, pair by pair (layout NS_ROTARY_*):
  *   (a, b) -> amplitude * (a cos t - b sin t, a sin t + b cos t),  t = pos[row] * freq[pair]  (inverse != 0: -t; with the same amplitude
  * that is the gradient), and the others copied.  Head h of row r is at x[r * x_ld + h * x_head], pitches in elements; y likewise, either x itself

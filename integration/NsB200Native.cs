@@ -318,6 +318,9 @@ internal static unsafe partial class NsB200Native
     public static partial int ns_attention_decode_quant(nint dev, nint cache, ulong q, long q_stride, ulong o, long o_stride, ulong page_table, int max_pages, ulong pos_dev, int batch, int steps, float scale, ulong q_out, ulong q_scale);
 
     [LibraryImport(Library)]
+    public static partial int ns_attention_shared(nint dev, nint cache, ulong q, long q_stride, ulong o, long o_stride, int heads, ulong prefix_table, int prefix_pages, ulong prefix_len, ulong page_table, int max_pages, ulong pos, ulong lens, int batch, int steps, float scale);
+
+    [LibraryImport(Library)]
     public static partial int ns_rotary(nint dev, ulong x, int dtype, long x_ld, long x_head, ulong pos, ulong freq, float amplitude, int layout, int inverse, long rows, int heads, int dim, int rot_dims, ulong y, long y_ld, long y_head);
 
     [LibraryImport(Library)]

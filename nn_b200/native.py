@@ -78,6 +78,7 @@ SIGNATURES = {
     "ns_kv_append": [vp, vp, u64, u64, i64, u64, i32, u64, i32, i32],
     "ns_attention_decode": [vp, vp, u64, i64, u64, i64, u64, i32, u64, i32, i32, f32],
     "ns_attention_prefill": [vp, u64, u64, u64, u64, i32, i32, i32, i32, P(i64), P(i64), P(i64), P(i64), f32, i32],
+    "ns_attention_shared": [vp, vp, u64, i64, u64, i64, i32, u64, i32, u64, u64, i32, u64, u64, i32, i32, f32],
     "ns_rotary": [vp, u64, i32, i64, i64, u64, u64, f32, i32, i32, i64, i32, i32, i32, u64, i64, i64],
     "ns_kv_append_rotary": [vp, vp, u64, i32, i32, i32, i32, i32, i32, i32, u64, f32, i32, i32, u64, u64, u64, u64, i32, i32, i32, u64, i64],
     "ns_linear_create": [vp, i32, i32, i32, P(f32), P(f32), i32, i32, i32, i32, P(vp)],

@@ -1,0 +1,336 @@
+"""ns_attention_shared against softmax attention in 64 bits.
+
+Tolerance of an output o = sum p_j v_j with normalised weights p: half a bf16 step of the result, 2^-8 |o|; the weights enter P.V rounded to bf16, half a step each,
+2^-8 sum p_j |v_j|; a score is a 32-bit sum of dim products, off by (dim + 4) 2^-24 sum |q k| scale, which shifts weights and their sum by that fraction,
+and exponentials, sums and folds add less than 2^-18: 2 ((dim + 4) 2^-24 max sum |q k| scale + 2^-18) sum p_j |v_j|."""
+import ctypes as C
+
+import numpy as np
+import pytest
+
+from nn_b200 import native as N
+
+from .test_rotary import _Cache, bf16, refused, values
+
+KEEP = 0x40E0      # 7: what an output holds before the call
+
+
+class Setup:
+    """A cache of random keys and values whose pages lie in any order, and what a call needs."""
+
+    def __init__(self, dev, dim, kv, group, page, batch, steps, prefix, own, seed=0, spare=3, std=1.0):
+        rng = self.rng = np.random.default_rng([dim, kv, group, page, batch, steps, prefix, max(own, default=0), seed])
+        self.dev, self.dim, self.kv, self.heads, self.page, self.batch, self.steps, self.prefix = dev, dim, kv, kv * group, page, batch, steps, prefix
+        self.pos = np.array(own, np.int32) - steps          # position of the first new token: the sequence has own[b] in all
+        self.prefix_pages = (prefix + page - 1) // page
+        self.max_pages = max((max(own, default=0) + page - 1) // page, 0)
+        n = self.prefix_pages + batch * self.max_pages + spare
+        order = rng.permutation(n).astype(np.int32)
+        self.prefix_table, self.table = order[:self.prefix_pages], order[self.prefix_pages:self.prefix_pages + batch * self.max_pages].reshape(batch, self.max_pages)
+        self.k, self.v = (bf16(std * rng.standard_normal((n, kv, page, dim)))[0] for _ in range(2))
+        self.q = bf16(rng.standard_normal((batch * steps, self.heads, dim)))[0]
+        self.scale = dim ** -0.5
+        self.lens = None
+        self.n_pages = n
+        self.cache = C.c_void_p()
+        N.call("ns_kv_cache_create", dev.handle, n, page, kv, dim, C.byref(self.cache))
+
+    def upload(self):
+        self.dev.synchronize()
+        for p, bits in zip(self.pools(), (self.k, self.v)):
+            N.call("ns_h2d", self.dev.handle, p, bits.ctypes.data_as(C.c_void_p), bits.nbytes)
+
+    def pools(self):
+        pools = [C.c_uint64(), C.c_uint64()]
+        N.call("ns_kv_cache_pools", self.cache, C.byref(pools[0]), C.byref(pools[1]), None)
+        return pools
+
+    def args(self, o_pad=0):
+        up = lambda a: self.dev.from_numpy(np.ascontiguousarray(a)) if a is not None and a.size else None
+        self.kept = [up(a) for a in (self.q.reshape(-1), self.prefix_table, np.array([self.prefix], np.int32), self.table, self.pos, self.lens)]
+        at = [0 if s is None else s.ptr for s in self.kept]
+        self.o_ld = self.heads * self.dim + o_pad
+        self.o = self.dev.from_numpy(np.full(self.batch * self.steps * self.o_ld, KEEP, np.uint16))
+        own = self.max_pages > 0
+        return (self.dev.handle, self.cache, at[0], self.heads * self.dim, self.o.ptr, self.o_ld, self.heads, at[1] if self.prefix_pages else 0, self.prefix_pages,
+                at[2] if self.prefix_pages else 0, at[3] if own else 0, self.max_pages, at[4] if own else 0, at[5], self.batch, self.steps, self.scale)
+
+    def call(self, o_pad=0):
+        N.call("ns_attention_shared", *self.args(o_pad))
+        self.dev.synchronize()
+        return self.read()
+
+    def read(self):
+        bits = self.o.download((self.batch * self.steps, self.o_ld))
+        assert (bits[:, self.heads * self.dim:] == KEEP).all()
+        return bits[:, :self.heads * self.dim].reshape(self.batch, self.steps, self.heads, self.dim)
+
+    def want(self):
+        """-> (outputs, tolerance) in 64 bits; NaN where the row is padding"""
+        k, v = values(self.k).astype(np.float64), values(self.v).astype(np.float64)
+        rows = lambda pool, table: pool[table].transpose(1, 0, 2, 3).reshape(self.kv, -1, self.dim)
+        q = values(self.q).astype(np.float64).reshape(self.batch, self.steps, self.kv, -1, self.dim)
+        out = np.full((self.batch, self.steps, self.kv, q.shape[3], self.dim), np.nan)
+        tol = np.zeros_like(out)
+        pk, pv = (rows(x, self.prefix_table)[:, :self.prefix] for x in (k, v))
+        for b in range(self.batch):
+            ok, ov = (rows(x, self.table[b]) for x in (k, v))
+            for i in range(self.steps):
+                if self.lens is not None and i >= self.lens[b]:
+                    continue
+                n = max(0, int(self.pos[b]) + i + 1) if self.max_pages else 0
+                kk, vv = np.concatenate([pk, ok[:, :n]], 1), np.concatenate([pv, ov[:, :n]], 1)
+                if kk.shape[1] == 0:
+                    out[b, i] = 0
+                    continue
+                s = np.einsum("kgd,kjd->kgj", q[b, i], kk) * self.scale
+                size = np.einsum("kgd,kjd->kgj", abs(q[b, i]), abs(kk)).max() * abs(self.scale)
+                w = np.exp(s - s.max(-1, keepdims=True))
+                w /= w.sum(-1, keepdims=True)
+                out[b, i] = w @ vv
+                tol[b, i] = 2.0 ** -8 * abs(out[b, i]) + (2.0 ** -8 + 2 * ((self.dim + 4) * 2.0 ** -24 * size + 2.0 ** -18)) * (w @ abs(vv))
+        shape = (self.batch, self.steps, self.heads, self.dim)
+        return out.reshape(shape), tol.reshape(shape)
+
+    def check(self, bits):
+        want, tol = self.want()
+        live = ~np.isnan(want)
+        assert (bits[~live] == KEEP).all()
+        got = values(bits).astype(np.float64)
+        assert not np.isnan(got).any()
+        far = np.where(live, abs(got - want) - tol, 0)
+        assert far.max() <= 0, (np.argwhere(far > 0)[:5], far.max())
+
+    def close(self):
+        N.call("ns_kv_cache_destroy", self.cache)
+
+
+CASES = [  # dim, kv heads, group, page, prefix, own positions of each sequence with the new ones, steps
+    (128, 2, 4, 64, 300, [40, 1, 130], 1),
+    (128, 1, 8, 16, 1, [1], 1),
+    (64, 2, 1, 16, 500, [37, 2, 19, 64], 1),
+    (32, 3, 2, 8, 129, [5, 200], 1),
+    (32, 1, 3, 4, 77, [9] * 20, 1),
+    (64, 1, 6, 1, 33, [3, 17], 2),
+    (128, 2, 2, 2, 50, [11, 12, 13], 4),
+    (64, 4, 4, 128, 1000, [130, 260, 7], 7),
+    (128, 1, 4, 32, 2000, [33] * 40, 1),            # 160 rows: more than one tile of any kernel
+    (128, 2, 8, 64, 700, [100] * 33, 1),            # 264 rows
+    (64, 1, 16, 16, 513, [65, 31] * 10, 3),
+    (32, 2, 4, 16, 4097, [300] * 16, 2),
+    (128, 8, 1, 16, 63, [1] * 5, 1),
+    (128, 1, 1, 16, 0, [100, 3], 1),                # no prefix
+    (64, 2, 4, 64, 0, [4000, 1, 700], 1),
+    (128, 2, 4, 16, 640, [], 1),                    # (filled in below: no pages of their own)
+    (32, 1, 40, 16, 200, [20, 25], 1),              # groups of more heads than a tile has rows
+    (128, 1, 2, 256, 900, [300, 20], 70),           # a portion of a prompt
+    (64, 2, 3, 64, 3000, [90] * 50, 1),
+]
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dim,kv,group,page,prefix,own,steps", CASES)
+def test_outputs(dev, dim, kv, group, page, prefix, own, steps):
+    s = Setup(dev, dim, kv, group, page, len(own) or 6, steps, prefix, own)
+    if not own:
+        s.pos = np.zeros(s.batch, np.int32)
+    s.upload()
+    s.check(s.call())
+    s.close()
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dim,page,batch", [(128, 64, 3), (64, 16, 40), (32, 8, 3), (128, 16, 70), (64, 4, 5)])
+def test_padding_and_rows_that_see_nothing(dev, dim, page, batch):
+    """Padded rows stay as they are; negative positions leave the prefix, without one zeros; positions beyond a table do not count; outputs with a gap."""
+    for prefix in (0, 75):
+        s = Setup(dev, dim, 2, 4, page, batch, 3, prefix, [41] * batch, seed=prefix)
+        s.lens = s.rng.integers(0, 4, batch).astype(np.int32)
+        s.pos = s.rng.integers(-4, 38, batch).astype(np.int32)
+        s.pos[0], s.lens[:3], s.pos[1], s.pos[2] = -2, 3, -2 ** 31, -3
+        s.upload()
+        s.check(s.call(o_pad=24))
+        s.pos[0], s.lens[:] = 2 ** 31 - 1, 3
+        bits = s.call()
+        s.pos[0] = s.max_pages * page - 1            # what it comes to: the whole table, for each of its tokens
+        want, tol = s.want()
+        assert (abs(values(bits[0, 0]) - want[0, 0]) <= tol[0, 0]).all()
+        s.close()
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dim,kv,group,page,batch,prefix", [(128, 2, 4, 64, 5, 300), (64, 1, 2, 16, 3, 65), (32, 2, 4, 4, 4, 130), (128, 1, 4, 16, 64, 1000), (64, 1, 4, 32, 50, 77)])
+def test_what_is_not_seen_does_not_count(dev, dim, kv, group, page, batch, prefix):
+    """Behind the last position of the prefix and of every sequence, and in pages nobody names: NaN, infinities, the type's lowest value."""
+    own = [1 + (7 * b) % 45 for b in range(batch)]
+    s = Setup(dev, dim, kv, group, page, batch, 1, prefix, own)
+    s.upload()
+    clean = s.call()
+    s.check(clean)
+    kept_k, kept_v = s.k.copy(), s.v.copy()
+    for bad in (0x7FC0, 0x7F80, 0xFF80, 0xFF7F):
+        k, v = np.full_like(s.k, bad), np.full_like(s.v, bad)
+        for table, n in [(s.prefix_table, prefix)] + [(s.table[b], own[b]) for b in range(batch)]:
+            for j in range(n):
+                k[table[j // page], :, j % page], v[table[j // page], :, j % page] = kept_k[table[j // page], :, j % page], kept_v[table[j // page], :, j % page]
+        s.k, s.v = k, v
+        s.upload()
+        assert np.array_equal(s.call(), clean)
+    s.close()
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dim,page,batch", [(128, 64, 2), (64, 16, 40), (128, 16, 70), (32, 16, 5)])
+def test_scores_that_are_no_numbers(dev, dim, page, batch):
+    """A NaN among the keys a row sees makes the row NaN, and only the rows that see it; a value of NaN too."""
+    for where in ("prefix", "own"):
+        for what in "kv":
+            s = Setup(dev, dim, 1, 4, page, batch, 1, 200, [50] * batch)
+            table, j = (s.prefix_table, 130) if where == "prefix" else (s.table[1], 20)
+            getattr(s, what)[table[j // page], 0, j % page, 3] = 0x7FC0
+            s.upload()
+            got = values(s.call())
+            touched = np.zeros(batch, bool)
+            touched[:] = where == "prefix"
+            touched[1] = True
+            assert np.isnan(got[touched][..., 3]).all() and (what == "v" or np.isnan(got[touched]).all())
+            assert not np.isnan(got[~touched]).any()
+            s.close()
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dim,page,batch,prefix", [(128, 16, 3, 100), (64, 64, 40, 500), (128, 32, 100, 1111), (32, 4, 4, 50)])
+def test_pages_outside_the_pool(dev, dim, page, batch, prefix):
+    """Positions of a page that is none are left out and reported."""
+    s = Setup(dev, dim, 2, 4, page, batch, 1, prefix, [60] * batch)
+    s.upload()
+    gone_p, gone_o = s.prefix_pages // 2, 0
+    s.prefix_table[gone_p] = s.n_pages
+    s.table[1, gone_o] = -1
+    N.call("ns_attention_shared", *s.args())
+    with pytest.raises(N.NsError) as e:
+        dev.synchronize()
+    assert e.value.code == 4
+    dev.synchronize()
+    got = s.read()
+    # the same without those positions: the tables closed up
+    full_table, full_pos = s.table, s.pos.copy()
+    s.prefix_table = np.delete(s.prefix_table, gone_p)
+    s.prefix -= page
+    want, tol = s.want()
+    for b in range(0, batch, 7):
+        assert b == 1 or (abs(values(got[b]) - want[b]) <= tol[b]).all()
+    s.table = np.concatenate([np.delete(full_table[1], gone_o), full_table[1][gone_o:gone_o + 1] * 0]).reshape(1, -1).repeat(batch, 0)
+    s.pos = full_pos - page if page <= 59 else np.full_like(full_pos, -1)
+    want, tol = s.want()
+    assert (abs(values(got[1]) - want[1]) <= tol[1]).all()
+    s.close()
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dim,group,batch", [(128, 4, 40), (64, 1, 3)])
+def test_values_alike(dev, dim, group, batch):
+    """Weights add up to one: values that are all alike come back within the rounding of the weights and of the output."""
+    s = Setup(dev, dim, 1, group, 64, batch, 1, 900, [70] * batch)
+    s.v[:] = bf16(np.broadcast_to(np.linspace(-3, 3, dim, dtype=np.float32), s.v.shape))[0]
+    s.upload()
+    got, want = values(s.call()).astype(np.float64), values(s.v[0, 0, 0]).astype(np.float64)
+    assert (abs(got - want) <= (2 * 2.0 ** -8 + 2.0 ** -16) * abs(want)).all()
+    s.close()
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("batch", [2, 40])
+def test_a_pool_of_more_than_2_31_elements(dev, batch):
+    dim, kv, page = 128, 8, 64
+    n = 2 ** 31 // (kv * page * dim) + 200
+    s = Setup(dev, dim, kv, 4, page, batch, 1, 200, [70] * batch)
+    N.call("ns_kv_cache_destroy", s.cache)
+    s.cache = C.c_void_p()
+    N.call("ns_kv_cache_create", dev.handle, n, page, kv, dim, C.byref(s.cache))
+    s.upload()                                       # the first pages
+    want = s.call()
+    s.check(want)
+    # the same pages at the pool's end
+    size = kv * page * dim * 2
+    for p, bits in zip(s.pools(), (s.k, s.v)):
+        N.call("ns_h2d", dev.handle, p.value + (n - s.n_pages) * size, bits.ctypes.data_as(C.c_void_p), bits.nbytes)
+    s.prefix_table, s.table = s.prefix_table + (n - s.n_pages), s.table + (n - s.n_pages)
+    assert np.array_equal(s.call(), want)
+    s.close()
+
+
+@pytest.mark.gpu
+def test_replays_with_other_lengths(dev):
+    """A recorded call follows the device's positions, length and tables; two recorded calls share the scratch block in stream order."""
+    sets = [Setup(dev, 128, 2, 4, 64, 6, 1, 500, [90] * 6, seed=1), Setup(dev, 64, 2, 4, 16, 40, 1, 300, [50] * 40, seed=2)]
+    graphs = []
+    for s in sets:
+        s.upload()
+        s.check(s.call())
+    for s in sets:
+        a = s.args()
+        dev.capture_begin()
+        N.call("ns_attention_shared", *a)
+        graphs.append(dev.capture_end())
+    for prefix, own in ((500, 90), (1, 1), (77, 30), (300, 50)):
+        for s in sets:
+            s.prefix, s.pos = min(prefix, s.prefix_pages * s.page), np.full(s.batch, min(own, s.max_pages * s.page) - 1, np.int32)
+            s.kept[2].upload(np.array([s.prefix], np.int32))
+            s.kept[4].upload(s.pos)
+        for g in graphs:
+            dev.graph_launch(g)
+        dev.synchronize()
+        for s in sets:
+            s.check(s.read())
+    for g in graphs:
+        dev.graph_destroy(g)
+    for s in sets:
+        s.close()
+
+
+@pytest.mark.gpu
+def test_runs_repeat_bit_for_bit(dev):
+    for batch in (3, 64):
+        s = Setup(dev, 128, 4, 4, 32, batch, 1, 3000, [200] * batch)
+        s.upload()
+        first = s.call()
+        for _ in range(3):
+            assert np.array_equal(s.call(), first)
+        s.close()
+
+
+def test_refusals():
+    A = 1 << 20
+    cache = _Cache(0, 8, 16, 2, 64, A, A, False)
+    good = dict(cache=C.addressof(cache), q=A, q_stride=512, o=A, o_stride=512, heads=8, prefix_table=A, prefix_pages=3, prefix_len=A, table=A, max_pages=2, pos=A, lens=0,
+                batch=2, steps=1, scale=0.1)
+
+    def call(text, **other):
+        refused(text, "ns_attention_shared", None, *{**good, **other}.values())
+
+    call("device handle is null")
+    call("device handle is null", batch=0)
+    call("device handle is null", prefix_pages=0, prefix_table=0, prefix_len=0)
+    call("device handle is null", max_pages=0, table=0, pos=0)
+    call("cache is null", cache=None)
+    call("null argument", q=0)
+    call("null argument", o=0)
+    call("without its table or length", prefix_table=0)
+    call("without its table or length", prefix_len=0)
+    call("without their table or positions", table=0)
+    call("without their table or positions", pos=0)
+    call("neither", prefix_pages=0, max_pages=0)
+    call("bad shape", batch=-1)
+    call("bad shape", prefix_pages=-1)
+    call("query heads", heads=0)
+    call("query heads", heads=7)
+    call("2^31 positions", prefix_pages=1 << 27)
+    call("2^31 positions", max_pages=1 << 27)
+    call("too many rows", batch=1 << 15, steps=1 << 15)
+    call("16-byte aligned", q=A + 8)
+    call("16-byte aligned", q_stride=516)
+    call("misaligned", pos=A + 2)
+    call("misaligned", o=A + 1)
+    call("shorter", q_stride=504)
+    call("shorter", o_stride=511)
