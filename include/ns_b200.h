@@ -365,9 +365,9 @@ NS_API int ns_attention_shared(ns_device_t dev, ns_kv_cache_t cache, uint64_t q,
 
 /* Rotary positions of query and key heads.  The first rot_dims columns of each head are turned, pair by pair (layout NS_ROTARY_*):
  *   (a, b) -> amplitude * (a cos t - b sin t, a sin t + b cos t),  t = pos[row] * freq[pair]  (inverse != 0: -t; with the same amplitude
- * that is the gradient), and the others copied.  Head h of row r is at x[r * x_ld + h * x_head], pitches in elements; y likewise, either x itself
+ * that is the gradient), and the others copied.  Head h of row r is at x[r * x_ld + h * x_head], pitches in elements (below 2^31); y likewise, either x itself
  * with x's pitches, or a matrix that does not overlap it.  x and y are both NS_F32 or NS_BF16; pos int32 [rows], rows of a negative position are
- * left as they are in y; freq float [rot_dims / 2].  t is computed in 64 bits, the rest in 32.  rot_dims even, dim <= 4096. */
+ * left as they are in y; freq float [rot_dims / 2].  t is computed in 64 bits, the rest in 32.  rot_dims even, dim <= 4096, heads * dim <= 2^19. */
 NS_API int ns_rotary(ns_device_t dev, uint64_t x, int dtype, int64_t x_ld, int64_t x_head, uint64_t pos, uint64_t freq, float amplitude, int layout,
                      int inverse, int64_t rows, int heads, int dim, int rot_dims, uint64_t y, int64_t y_ld, int64_t y_head);
 

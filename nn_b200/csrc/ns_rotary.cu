@@ -17,10 +17,11 @@ namespace {
 
 constexpr int ROT_THREADS = 256;
 constexpr int ROT_MAX_DIM = 4096;
+constexpr int ROT_MAX_COLUMNS = 1 << 19;
 
 // amplitude * (cos, sin) of position * freq.  The angle in turns, reduced to half a turn either way, in 64 bits; its doubled value as a float and the
 // rest of it, which moves the result along its derivative: within an ulp or two of the exact value.
-__device__ __forceinline__ float2 rot_cos_sin(double position, float freq, float amplitude)
+__device__ __forceinline__ float2 rot_cos_sin(double position, float freq, float amplitude, float sign = 1.0f)
 {
     double turns = position * (double)freq * 0.15915494309189535;
     turns -= rint(turns);
@@ -28,7 +29,7 @@ __device__ __forceinline__ float2 rot_cos_sin(double position, float freq, float
     const float hi = (float)twice, lo = (float)(twice - (double)hi) * 3.14159274f;
     float s, c;
     sincospif(hi, &s, &c);
-    return make_float2(amplitude * fmaf(-lo, s, c), amplitude * fmaf(lo, c, s));
+    return make_float2(amplitude * fmaf(-lo, s, c), sign * amplitude * fmaf(lo, c, s));
 }
 
 template <typename T, int VEC>
@@ -36,69 +37,113 @@ struct alignas(sizeof(T) * VEC) RotVec {
     T v[VEC];
 };
 
-__device__ __forceinline__ float rot_float(float v) { return v; }
-__device__ __forceinline__ float rot_float(uint16_t v) { return ns_bf16_bits_to_f32(v); }
-__device__ __forceinline__ void rot_put(float& d, float v) { d = v; }
-__device__ __forceinline__ void rot_put(uint16_t& d, float v) { d = ns_f32_to_bf16_bits(v); }
-
-// How a head's columns are dealt out.  A task is VEC neighbouring pairs of halves, or VEC neighbouring columns (pairs of neighbours lie inside; columns
-// behind the turned ones are copied).
-template <bool HALVES, int VEC>
-struct RotTasks {
-    int half, dim, turned, per_head;      // turned: tasks that turn something
-    __host__ __device__ RotTasks(int dim_, int rot, bool copies) : half(rot / 2), dim(dim_)
-    {
-        if (HALVES) {
-            turned = half / VEC;
-            per_head = turned + (copies ? (dim - rot) / VEC : 0);
-        } else {
-            // (scalar: a task is a pair, then single columns)
-            const int columns = VEC > 1 ? VEC : 2;
-            turned = (rot + columns - 1) / columns;
-            per_head = copies ? (VEC > 1 ? dim / VEC : half + dim - rot) : turned;
-        }
-    }
-    // first column of a task, and of its second vector
-    __device__ __forceinline__ int first(int t) const
-    {
-        if (HALVES) return t < turned ? t * VEC : 2 * half + (t - turned) * VEC;
-        if (VEC == 1) return t < turned ? 2 * t : 2 * half + (t - turned);
-        return t * VEC;
-    }
-};
-
-// the columns of one task in 32 bits: a, and for halves or scalar pairs b
-template <bool HALVES, int VEC>
-__device__ __forceinline__ void rot_turn(const RotTasks<HALVES, VEC>& n, int t, const float2* cs, float sign, float (&a)[VEC], float (&b)[VEC])
+template <int VEC>
+__device__ __forceinline__ void rot_unpack(const RotVec<float, VEC>& x, float (&f)[VEC])
 {
-    if (t >= n.turned) return;
-    if (HALVES || VEC == 1) {
 #pragma unroll
-        for (int i = 0; i < VEC; i++) {
-            const float2 w = cs[t * VEC + i];
-            const float x = a[i], y = b[i], s = sign * w.y;
-            a[i] = fmaf(x, w.x, -(y * s));
-            b[i] = fmaf(x, s, y * w.x);
-        }
+    for (int i = 0; i < VEC; i++) f[i] = x.v[i];
+}
+template <int VEC>
+__device__ __forceinline__ void rot_unpack(const RotVec<uint16_t, VEC>& x, float (&f)[VEC])
+{
+    if constexpr (VEC == 1) {
+        f[0] = ns_bf16_bits_to_f32(x.v[0]);
     } else {
+        const uint32_t* w = reinterpret_cast<const uint32_t*>(&x);
 #pragma unroll
-        for (int i = 0; i + 1 < VEC; i += 2) {
-            const int p = (t * VEC + i) >> 1;
-            if (p < n.half) {
-                const float2 w = cs[p];
-                const float x = a[i], y = a[i + 1], s = sign * w.y;
-                a[i] = fmaf(x, w.x, -(y * s));
-                a[i + 1] = fmaf(x, s, y * w.x);
-            }
+        for (int i = 0; i < VEC / 2; i++) {
+            f[2 * i] = __uint_as_float(w[i] << 16);
+            f[2 * i + 1] = __uint_as_float(w[i] & 0xFFFF0000u);
         }
     }
 }
+template <int VEC>
+__device__ __forceinline__ void rot_pack(RotVec<float, VEC>& x, const float (&f)[VEC])
+{
+#pragma unroll
+    for (int i = 0; i < VEC; i++) x.v[i] = f[i];
+}
+template <int VEC>
+__device__ __forceinline__ void rot_pack(RotVec<uint16_t, VEC>& x, const float (&f)[VEC])
+{
+    if constexpr (VEC == 1) {
+        x.v[0] = ns_f32_to_bf16_bits(f[0]);
+    } else {
+        uint32_t* w = reinterpret_cast<uint32_t*>(&x);
+#pragma unroll
+        for (int i = 0; i < VEC / 2; i++) w[i] = ns_pack_bf16x2(f[2 * i], f[2 * i + 1]);
+    }
+}
 
-// whether a task has a second vector, and where it is
+// How a head's columns are dealt out.  A task turns PAIRS neighbouring pairs: VEC neighbouring columns of each half, VEC neighbouring columns that hold VEC / 2
+// pairs (the last task may hold columns behind the turned ones), or, column by column, one pair.  The columns from `rest` on are copied.
 template <bool HALVES, int VEC>
-__device__ __forceinline__ bool rot_second(const RotTasks<HALVES, VEC>& n, int t) { return (HALVES || VEC == 1) && t < n.turned; }
-template <bool HALVES, int VEC>
-__device__ __forceinline__ int rot_second_at(const RotTasks<HALVES, VEC>& n, int c) { return HALVES ? c + n.half : c + 1; }
+struct RotTasks {
+    static constexpr int PAIRS = HALVES || VEC == 1 ? VEC : VEC / 2;
+    static constexpr bool TWO = HALVES || VEC == 1;                       // two vectors a task
+    int half, turned, rest;
+    __host__ __device__ RotTasks(int dim, int rot) : half(rot / 2), turned((rot / 2 + PAIRS - 1) / PAIRS), rest(TWO ? rot : turned * VEC) {}
+    __device__ __forceinline__ int first(int t) const { return HALVES ? t * VEC : t * (VEC == 1 ? 2 : VEC); }
+    __device__ __forceinline__ int second() const { return HALVES ? half : 1; }      // from the first vector's column to the second's
+    // Where a row's cosine and sine of pair p lie: neighbouring tasks' side by side, so that neighbouring threads read them without conflicts.
+    __host__ __device__ int table() const { return PAIRS * turned; }
+    __device__ __forceinline__ int slot(int p) const { return p % PAIRS * turned + p / PAIRS; }
+    __device__ __forceinline__ void angles(const float2* row, int t, float2 (&w)[PAIRS]) const
+    {
+#pragma unroll
+        for (int i = 0; i < PAIRS; i++) w[i] = row[i * turned + t];
+    }
+    // the columns of task t in 32 bits
+    __device__ __forceinline__ void turn(int t, const float2 (&w)[PAIRS], float (&a)[VEC], float (&b)[VEC]) const
+    {
+        const int live = half - t * PAIRS;
+#pragma unroll
+        for (int i = 0; i < PAIRS; i++) {
+            float& x = TWO ? a[i] : a[(2 * i) % VEC];
+            float& y = TWO ? b[i] : a[(2 * i + 1) % VEC];
+            const float u = x, v = y;
+            if (TWO || i < live) {
+                x = fmaf(u, w[i].x, -(v * w[i].y));
+                y = fmaf(u, w[i].y, v * w[i].x);
+            }
+        }
+    }
+};
+
+// How a CTA's threads are dealt out: `tasks` threads a head, `heads` of them at a time, `rows` of those; a thread keeps its pairs' cosines and sines in registers
+// and walks heads.
+struct RotLanes {
+    int tasks, heads, rows;
+};
+RotLanes rot_lanes(const NsDevice* d, int64_t rows, int heads, int turned, int table, int columns)
+{
+    RotLanes best{turned < ROT_THREADS ? turned : ROT_THREADS, 1, 1};
+    const int slots = ROT_THREADS / best.tasks;
+    // few rows: all heads at once.  Else the fewest idle threads, with four to eight heads a thread where that is level.
+    if (rows < 2 * d->sm_count) {
+        best.heads = heads < slots ? heads : slots;
+        return best;
+    }
+    double most = 0.0;
+    for (int h = 1; h <= slots && h <= heads; h++) {
+        int r = slots / h;
+        if ((int64_t)r * table > 2048) r = 2048 / table > 1 ? 2048 / table : 1;
+        if (r > (1 << 16) / columns) r = (1 << 16) / columns > 1 ? (1 << 16) / columns : 1;       // (RotDiv)
+        if (r > rows / (4 * d->sm_count)) r = (int)(rows / (4 * d->sm_count));
+        if (r < 1) r = 1;
+        const int walk = (heads + h - 1) / h;
+        const double busy = (double)r * heads * best.tasks / ((double)walk * ROT_THREADS) * (walk < 4 ? 0.8 + 0.05 * walk : walk > 8 ? 0.9 : 1.0);
+        if (busy > most) { most = busy; best.heads = h; best.rows = r; }
+    }
+    return best;
+}
+
+// n / d, exact while n * d < 2^32 (m d - 2^32 < d)
+struct RotDiv {
+    uint32_t d, m;
+    explicit RotDiv(int divisor = 0) : d((uint32_t)divisor), m(divisor > 1 ? (uint32_t)(((1ull << 32) + divisor - 1) / divisor) : 0u) {}
+    __device__ __forceinline__ int of(int n) const { return d == 1 ? n : (int)__umulhi((uint32_t)n, m); }
+};
 
 // ---------------------------------------------------------------------------------------------
 // rows of a matrix
@@ -106,82 +151,105 @@ __device__ __forceinline__ int rot_second_at(const RotTasks<HALVES, VEC>& n, int
 struct RotaryArgs {
     const void* x;
     void* y;
-    int64_t x_ld, x_head, y_ld, y_head;
+    int x_ld, x_head, y_ld, y_head;
     const int32_t* pos;
     const float* freq;
     float amplitude, sign;
     int64_t rows;
-    int heads, dim, rot;
+    int dim, rot;
     int copies;            // y is another matrix: the columns that are not turned are copied
-    int group;             // threads a row
-    int heads_each;        // heads a CTA takes of its rows (blockIdx.y)
+    int heads, heads_each; // heads a CTA takes of its rows (blockIdx.y)
+    RotLanes lanes;
+    RotDiv half, rest, rest_row;         // pairs of a row, vectors of a head and of a row that are copied
 };
 
+// A CTA takes a few rows: their first columns are asked for, the cosines and sines of all the rows computed meanwhile, one or two a thread, and then
+// the rows' heads stream through.
 template <typename T, bool HALVES, int VEC>
-__global__ void __launch_bounds__(ROT_THREADS) ns_rotary_kernel(const RotaryArgs p)
+__global__ void __launch_bounds__(ROT_THREADS, 4) ns_rotary_kernel(const RotaryArgs p)
 {
-    constexpr int U = VEC >= 4 ? 2 : 4;      // tasks in flight
     using V = RotVec<T, VEC>;
+    using N = RotTasks<HALVES, VEC>;
+    constexpr int U = N::TWO ? 2 : 4;          // heads a thread has on their way
     extern __shared__ float2 rot_table[];
     ns_pdl_wait();
     ns_pdl_trigger();
-    const RotTasks<HALVES, VEC> n(p.dim, p.rot, p.copies != 0);
-    const int per_cta = ROT_THREADS / p.group, slot = threadIdx.x / p.group, lane = threadIdx.x % p.group;
-    const int half = p.rot / 2;
-    float2* cs = rot_table + slot * half;
-    const int h0 = blockIdx.y * p.heads_each, heads = min(p.heads_each, p.heads - h0);
-    const int tasks = heads * n.per_head;
-    for (int64_t r0 = (int64_t)blockIdx.x * per_cta; r0 < p.rows; r0 += (int64_t)gridDim.x * per_cta) {
-        const int64_t r = r0 + slot;
-        const int pos = r < p.rows ? p.pos[r] : -1;
-        const T* x = reinterpret_cast<const T*>(p.x) + r * p.x_ld + h0 * p.x_head;
-        T* y = reinterpret_cast<T*>(p.y) + r * p.y_ld + h0 * p.y_head;
-        bool table = false;
-        // (the loop runs once at least in every thread: the barrier stands in it)
-        for (int at = lane; at < tasks || !table; at += U * p.group) {
-            V a[U], b[U];
-            int head[U], task[U];
+    const N n(p.dim, p.rot);
+    const int half = p.rot / 2, h0 = blockIdx.y * p.heads_each, heads = min(p.heads_each, p.heads - h0);
+    const int slot = threadIdx.x / p.lanes.tasks, t0 = threadIdx.x - slot * p.lanes.tasks, my_row = slot / p.lanes.heads, my_head = slot - my_row * p.lanes.heads;
+    for (int64_t r0 = (int64_t)blockIdx.x * p.lanes.rows; r0 < p.rows; r0 += (int64_t)gridDim.x * p.lanes.rows) {
+        const int rows = (int)min((int64_t)p.lanes.rows, p.rows - r0);
+        const int32_t* pos = p.pos + r0;
+        const T* x0 = reinterpret_cast<const T*>(p.x) + r0 * p.x_ld + (int64_t)h0 * p.x_head;
+        T* y0 = reinterpret_cast<T*>(p.y) + r0 * p.y_ld + (int64_t)h0 * p.y_head;
+        const T* x = x0 + (int64_t)my_row * p.x_ld;
+        T* y = y0 + (int64_t)my_row * p.y_ld;
+        const bool mine = my_row < rows;
+        V a[U], b[U];
+        auto load = [&](int t, int h) {
 #pragma unroll
             for (int u = 0; u < U; u++) {
-                const int e = at + u * p.group;
-                head[u] = e / n.per_head;
-                task[u] = e - head[u] * n.per_head;
-                if (e < tasks && pos >= 0) {
-                    const T* src = x + head[u] * p.x_head;
-                    const int c = n.first(task[u]);
-                    a[u] = *reinterpret_cast<const V*>(src + c);
-                    if (rot_second(n, task[u])) b[u] = *reinterpret_cast<const V*>(src + rot_second_at(n, c));
+                const int head = h + u * p.lanes.heads;
+                if (head < heads) {
+                    const T* src = x + (int64_t)head * p.x_head + n.first(t);
+                    a[u] = *reinterpret_cast<const V*>(src);
+                    if (N::TWO) b[u] = *reinterpret_cast<const V*>(src + n.second());
                 }
             }
-            if (!table) {
-                __syncthreads();       // the row before has been turned
-                if (pos >= 0)
-                    for (int i = lane; i < half; i += p.group) cs[i] = rot_cos_sin((double)pos, p.freq[i], p.amplitude);
-                __syncthreads();
-                table = true;
+        };
+        if (mine) load(t0, my_head);
+        if (p.copies != 0 && n.rest < p.dim) {
+            const int per_head = (p.dim - n.rest) / VEC, per_row = heads * per_head;
+            constexpr int C = 4;
+            for (int e = threadIdx.x; e < rows * per_row; e += C * ROT_THREADS) {
+                V v[C];
+                T* to[C];
+#pragma unroll
+                for (int u = 0; u < C; u++) {
+                    const int i = e + u * ROT_THREADS, r = rows == 1 ? 0 : p.rest_row.of(i), in = i - r * per_row, head = p.rest.of(in);
+                    const int c = n.rest + (in - head * per_head) * VEC;
+                    to[u] = nullptr;
+                    if (i < rows * per_row && pos[r] >= 0) {
+                        v[u] = *reinterpret_cast<const V*>(x0 + (int64_t)r * p.x_ld + (int64_t)head * p.x_head + c);
+                        to[u] = y0 + (int64_t)r * p.y_ld + (int64_t)head * p.y_head + c;
+                    }
+                }
+#pragma unroll
+                for (int u = 0; u < C; u++)
+                    if (to[u] != nullptr) *reinterpret_cast<V*>(to[u]) = v[u];
             }
+        }
+        __syncthreads();                       // the rows before have been turned
+        for (int i = threadIdx.x; i < rows * half; i += ROT_THREADS) {
+            const int r = p.half.of(i), pair = i - r * half;
+            rot_table[r * n.table() + n.slot(pair)] = rot_cos_sin((double)pos[r], p.freq[pair], p.amplitude, p.sign);
+        }
+        __syncthreads();
+        if (mine && pos[my_row] >= 0) {
+            for (int t = t0; t < n.turned; t += p.lanes.tasks) {
+                float2 w[N::PAIRS];
+                n.angles(rot_table + my_row * n.table(), t, w);
+                if (t != t0) load(t, my_head);
+                for (int h = my_head; h < heads; h += U * p.lanes.heads) {
 #pragma unroll
-            for (int u = 0; u < U; u++) {
-                if (at + u * p.group < tasks && pos >= 0) {
-                    float fa[VEC], fb[VEC];
-                    const bool second = rot_second(n, task[u]);
-#pragma unroll
-                    for (int i = 0; i < VEC; i++) {
-                        fa[i] = rot_float(a[u].v[i]);
-                        fb[i] = second ? rot_float(b[u].v[i]) : 0.0f;
+                    for (int u = 0; u < U; u++) {
+                        const int head = h + u * p.lanes.heads;
+                        if (head < heads) {
+                            float fa[VEC], fb[VEC];
+                            rot_unpack(a[u], fa);
+                            if (N::TWO) rot_unpack(b[u], fb);
+                            n.turn(t, w, fa, fb);
+                            V o;
+                            T* dst = y + (int64_t)head * p.y_head + n.first(t);
+                            rot_pack(o, fa);
+                            *reinterpret_cast<V*>(dst) = o;
+                            if (N::TWO) {
+                                rot_pack(o, fb);
+                                *reinterpret_cast<V*>(dst + n.second()) = o;
+                            }
+                        }
                     }
-                    rot_turn(n, task[u], cs, p.sign, fa, fb);
-                    V oa, ob;
-#pragma unroll
-                    for (int i = 0; i < VEC; i++) {
-                        rot_put(oa.v[i], fa[i]);
-                        rot_put(ob.v[i], fb[i]);
-                    }
-                    T* dst = y + head[u] * p.y_head;
-                    const int c = n.first(task[u]);
-                    // columns that are not turned keep their bits
-                    *reinterpret_cast<V*>(dst + c) = task[u] < n.turned ? oa : a[u];
-                    if (second) *reinterpret_cast<V*>(dst + rot_second_at(n, c)) = ob;
+                    load(t, h + U * p.lanes.heads);
                 }
             }
         }
@@ -212,14 +280,6 @@ int rot_pick(bool halves, int vec, F f)
     return halves ? by(std::true_type()) : by(std::false_type());
 }
 
-// threads a row: as many as it has tasks, a warp at least and a CTA at most
-int rot_group(int64_t tasks)
-{
-    int g = 32;
-    while (g < ROT_THREADS && g < tasks) g *= 2;
-    return g;
-}
-
 // ---------------------------------------------------------------------------------------------
 // into the cache
 // ---------------------------------------------------------------------------------------------
@@ -238,90 +298,143 @@ struct AppendArgs {
     int64_t q_ld;
     uint16_t* k_pool;
     uint16_t* v_pool;
-    int group, tasks_each;
+    int lane_tasks;                        // lanes a head, at most 32
+    int parts;                             // warps a row, each a share of its heads and vectors
+    RotDiv rest, value;                    // vectors of a head that are not turned, and of a value head
     int* status;
 };
 
-// VEC values of the source from element idx on, in 32 bits
+// VEC neighbouring values of the source as they are held until they are used: bf16 as it lies there, float slabs as their sum.
+constexpr int ROT_BF16 = -1;               // in place of a number of slabs
 template <int VEC, int SLABS>
-__device__ __forceinline__ void rot_source(const NsSource& s, int64_t idx, float (&v)[VEC])
+using RotHeld = typename std::conditional<SLABS == ROT_BF16, RotVec<uint16_t, VEC>, RotVec<float, VEC>>::type;
+template <int VEC, int SLABS>
+__device__ __forceinline__ void rot_source(const NsSource& s, int64_t idx, RotHeld<VEC, SLABS>& v)
 {
-    if constexpr (VEC % 4 == 0) {
+    if constexpr (SLABS == ROT_BF16) {
+        v = *reinterpret_cast<const RotVec<uint16_t, VEC>*>(reinterpret_cast<const uint16_t*>(s.ptr) + idx);
+    } else if constexpr (VEC % 4 == 0) {
 #pragma unroll
         for (int i = 0; i < VEC; i += 4) {
             const float4 f = ns_source_at4<SLABS>(s, idx + i);
-            v[i] = f.x; v[i + 1] = f.y; v[i + 2] = f.z; v[i + 3] = f.w;
+            v.v[i] = f.x; v.v[i + 1] = f.y; v.v[i + 2] = f.z; v.v[i + 3] = f.w;
         }
     } else {
 #pragma unroll
-        for (int i = 0; i < VEC; i++) v[i] = ns_source_at<SLABS>(s, idx + i);
+        for (int i = 0; i < VEC; i++) v.v[i] = ns_source_at<SLABS>(s, idx + i);
     }
 }
 template <int VEC>
-__device__ __forceinline__ void rot_store(uint16_t* dst, const float (&v)[VEC])
+__device__ __forceinline__ void rot_store(uint16_t* dst, const RotVec<uint16_t, VEC>& v) { *reinterpret_cast<RotVec<uint16_t, VEC>*>(dst) = v; }
+template <int VEC>
+__device__ __forceinline__ void rot_store(uint16_t* dst, const RotVec<float, VEC>& v)
 {
     RotVec<uint16_t, VEC> o;
-#pragma unroll
-    for (int i = 0; i < VEC; i++) o.v[i] = ns_f32_to_bf16_bits(v[i]);
-    *reinterpret_cast<RotVec<uint16_t, VEC>*>(dst) = o;
+    rot_pack(o, v.v);
+    rot_store<VEC>(dst, o);
 }
 
+// A warp a row, or several where there are few rows; no barrier joins them.  What a token's place and angles come from is a chain of three loads (position, page, data), so what
+// counts is that many warps are at different links of it.
 template <bool HALVES, int VEC, int SLABS>
-__global__ void __launch_bounds__(ROT_THREADS) ns_kv_append_rotary_kernel(const AppendArgs p)
+__global__ void __launch_bounds__(ROT_THREADS, SLABS == NS_TOGETHER ? 1 : SLABS == ROT_BF16 ? 4 : 3) ns_kv_append_rotary_kernel(const AppendArgs p)
 {
+    using N = RotTasks<HALVES, VEC>;
+    using H = RotHeld<VEC, SLABS>;
+    constexpr int U = SLABS == NS_TOGETHER ? 1 : SLABS == ROT_BF16 && !N::TWO ? 4 : 2;      // heads a lane has on their way
+    constexpr int K = SLABS == NS_TOGETHER ? 1 : SLABS == ROT_BF16 ? 4 : 2;                 // vectors to copy
     extern __shared__ float2 rot_table[];
     ns_pdl_wait();
     ns_pdl_trigger();
-    const RotTasks<HALVES, VEC> n(p.dim, p.rot, true);
-    const int per_cta = ROT_THREADS / p.group, slot = threadIdx.x / p.group, lane = threadIdx.x % p.group;
-    const int half = p.rot / 2;
-    float2* cs = rot_table + slot * half;
-    const int rows = p.batch * p.steps;
-    // tasks of a row: the query heads', the key heads', then the values' columns
-    const int turned = (p.heads + p.kv_heads) * n.per_head, tasks = turned + p.kv_heads * (p.dim / VEC);
-    const int first = blockIdx.y * p.tasks_each, end = min(first + p.tasks_each, tasks);
-    const int page_size = 1 << p.page_shift;
-    const int offset = p.offset != nullptr ? p.offset[0] : 0;
-    for (int r0 = blockIdx.x * per_cta; r0 < rows; r0 += gridDim.x * per_cta) {
-        const int r = r0 + slot;
-        const int b = r / p.steps, i = r - b * p.steps;
-        const bool live = r < rows && (p.lens == nullptr || i < p.lens[b]);
-        // positions in 64 bits: nothing a caller leaves in a padded row wraps around
-        const int64_t at = live ? (int64_t)p.pos[b] + i : 0;
-        __syncthreads();
-        if (live)
-            for (int e = lane; e < half; e += p.group) cs[e] = rot_cos_sin((double)(at + offset), p.freq[e], p.amplitude);
-        __syncthreads();
-        if (!live) continue;
-        int page = -1;
-        if (at >= 0 && (at >> p.page_shift) < p.max_pages) page = p.page_table[(int64_t)b * p.max_pages + (at >> p.page_shift)];
-        const bool stored = page >= 0 && page < p.num_pages;
-        if (!stored && lane == 0) *reinterpret_cast<volatile int*>(p.status) = 500;
-        const int64_t row = (int64_t)r * p.src.ld;
-        const int64_t slab = ((int64_t)page * p.kv_heads * page_size + (at & (page_size - 1))) * p.dim;      // head 0's row in the page
-        const int64_t head_step = (int64_t)page_size * p.dim;
-        for (int e = first + lane; e < end; e += p.group) {
-            float a[VEC], c[VEC];
-            if (e < turned) {
-                const int head = e / n.per_head, t = e - head * n.per_head, col = n.first(t);
-                const bool key = head >= p.heads;
-                if (key && !stored) continue;
-                const int64_t src = row + (key ? p.k_col + (head - p.heads) * p.dim : p.q_col + head * p.dim) + col;
-                uint16_t* dst = key ? p.k_pool + slab + (head - p.heads) * head_step + col : p.q + (int64_t)r * p.q_ld + (int64_t)head * p.dim + col;
-                rot_source<VEC, SLABS>(p.src, src, a);
-                const bool second = rot_second(n, t);
-                const int step = rot_second_at(n, col) - col;
-                if (second) rot_source<VEC, SLABS>(p.src, src + step, c);
-                rot_turn(n, t, cs, 1.0f, a, c);
-                rot_store<VEC>(dst, a);
-                if (second) rot_store<VEC>(dst + step, c);
-            } else if (stored) {
-                const int per = p.dim / VEC, head = (e - turned) / per, col = (e - turned - head * per) * VEC;
-                rot_source<VEC, SLABS>(p.src, row + p.v_col + head * p.dim + col, a);
-                rot_store<VEC>(p.v_pool + slab + head * head_step + col, a);
+    const N n(p.dim, p.rot);
+    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, half = p.rot / 2;
+    const int item = blockIdx.x * (ROT_THREADS / 32) + warp, r = item / p.parts, part = item - r * p.parts;
+    if (r >= p.batch * p.steps) return;
+    const int b = r / p.steps, i = r - b * p.steps;
+    const int first_pos = p.pos[b], offset = p.offset != nullptr ? p.offset[0] : 0;
+    if (p.lens != nullptr && i >= p.lens[b]) return;
+    // positions in 64 bits: nothing wraps around
+    const int64_t at = (int64_t)first_pos + i;
+    int page = -1;
+    if (at >= 0 && (at >> p.page_shift) < p.max_pages) page = p.page_table[(int64_t)b * p.max_pages + (at >> p.page_shift)];
+    const int64_t src0 = (int64_t)r * p.src.ld, head_step = (int64_t)p.dim << p.page_shift;
+
+    // ---- turned heads: lanes of a head, heads side by side
+    const int across = 32 / p.lane_tasks, t0 = lane % p.lane_tasks, sub = lane / p.lane_tasks, step = across * p.parts;
+    const int all_heads = p.heads + p.kv_heads;
+    auto source = [&](int head) { return src0 + (head < p.heads ? p.q_col + head * p.dim : p.k_col + (head - p.heads) * p.dim); };
+    H x[U], y[U];
+    auto load = [&](int t, int h) {
+#pragma unroll
+        for (int u = 0; u < U; u++)
+            if (h + u * step < all_heads) {
+                const int64_t src = source(h + u * step) + n.first(t);
+                rot_source<VEC, SLABS>(p.src, src, x[u]);
+                if (N::TWO) rot_source<VEC, SLABS>(p.src, src + n.second(), y[u]);
+            }
+    };
+    const bool mine = sub < across;
+    const int h0 = part * across + sub;
+    if (mine) load(t0, h0);
+    float2* table = rot_table + warp * n.table();
+    for (int e = lane; e < half; e += 32) table[n.slot(e)] = rot_cos_sin((double)(at + offset), p.freq[e], p.amplitude);
+    __syncwarp();
+    const bool stored = page >= 0 && page < p.num_pages;
+    if (!stored && lane == 0) *reinterpret_cast<volatile int*>(p.status) = 500;
+    const int64_t slab = (((int64_t)page * p.kv_heads << p.page_shift) + (at & ((1 << p.page_shift) - 1))) * p.dim;      // head 0's row in the page
+    auto target = [&](int head) { return head < p.heads ? p.q + (int64_t)r * p.q_ld + (int64_t)head * p.dim : p.k_pool + slab + (int64_t)(head - p.heads) * head_step; };
+    const int heads = stored ? all_heads : p.heads;
+    if (mine) {
+        for (int t = t0; t < n.turned; t += p.lane_tasks) {
+            float2 w[N::PAIRS];
+            n.angles(table, t, w);
+            if (t != t0) load(t, h0);
+            for (int h = h0; h < heads; h += U * step) {
+#pragma unroll
+                for (int u = 0; u < U; u++)
+                    if (h + u * step < heads) {
+                        uint16_t* dst = target(h + u * step) + n.first(t);
+                        float fa[VEC], fb[VEC];
+                        rot_unpack(x[u], fa);
+                        if (N::TWO) rot_unpack(y[u], fb);
+                        n.turn(t, w, fa, fb);
+                        RotVec<uint16_t, VEC> o;
+                        rot_pack(o, fa);
+                        rot_store<VEC>(dst, o);
+                        if (N::TWO) {
+                            rot_pack(o, fb);
+                            rot_store<VEC>(dst + n.second(), o);
+                        }
+                    }
+                load(t, h + U * step);
             }
         }
     }
+    // ---- what is not turned of those heads, and the values
+    H v[K];
+    auto copy = [&](int count, auto where) {
+        for (int e = part * 32 + lane; e < count; e += K * 32 * p.parts) {
+            uint16_t* to[K];
+#pragma unroll
+            for (int u = 0; u < K; u++)
+                if (e + u * 32 * p.parts < count) rot_source<VEC, SLABS>(p.src, where(e + u * 32 * p.parts, to[u]), v[u]);
+#pragma unroll
+            for (int u = 0; u < K; u++)
+                if (e + u * 32 * p.parts < count) rot_store<VEC>(to[u], v[u]);
+        }
+    };
+    const int rest = (p.dim - n.rest) / VEC;
+    copy(heads * rest, [&](int e, uint16_t*& to) {
+        const int head = p.rest.of(e), c = n.rest + (e - head * rest) * VEC;
+        to = target(head) + c;
+        return source(head) + c;
+    });
+    const int per = p.dim / VEC;
+    copy(stored ? p.kv_heads * per : 0, [&](int e, uint16_t*& to) {
+        const int head = p.value.of(e), c = (e - head * per) * VEC;
+        to = p.v_pool + slab + head * head_step + c;
+        return src0 + p.v_col + head * p.dim + c;
+    });
 }
 
 bool rot_layout(int layout) { return layout == NS_ROTARY_PAIRS || layout == NS_ROTARY_HALVES; }
@@ -339,13 +452,14 @@ extern "C" int ns_rotary(ns_device_t h, uint64_t x, int dtype, int64_t x_ld, int
     NS_REQUIRE(((pos | freq) & 3) == 0, NS_ERR_ARGUMENT, "ns_rotary: pos and freq must be 4-byte aligned");
     const int size = dtype == NS_F32 ? 4 : 2;
     NS_REQUIRE(((x | y) & (uint64_t)(size - 1)) == 0, NS_ERR_ARGUMENT, "ns_rotary: rows must be aligned to their type");
-    NS_REQUIRE((int64_t)heads * dim <= (1 << 24), NS_ERR_ARGUMENT, "ns_rotary: at most 2^24 columns a row");
+    NS_REQUIRE((int64_t)heads * dim <= ROT_MAX_COLUMNS, NS_ERR_ARGUMENT, "ns_rotary: at most 2^19 columns a row");
     // no two (row, head) of the output share a column: heads inside rows, or rows inside heads
     auto apart = [&](int64_t inner, int64_t n_inner, int64_t outer, int64_t n_outer) {
         const bool in = n_inner == 1 || inner >= dim;
         return in && (n_outer == 1 || (outer >= dim && (n_inner == 1 || (outer - dim) / inner >= n_inner - 1)));
     };
     NS_REQUIRE(x_ld >= 0 && x_head >= 0 && y_ld >= 0 && y_head >= 0, NS_ERR_ARGUMENT, "ns_rotary: negative pitch");
+    NS_REQUIRE(x_ld < (1LL << 31) && x_head < (1LL << 31) && y_ld < (1LL << 31) && y_head < (1LL << 31), NS_ERR_ARGUMENT, "ns_rotary: a pitch of 2^31 elements or more");
     NS_REQUIRE(apart(y_head, heads, y_ld, rows) || apart(y_ld, rows, y_head, heads), NS_ERR_ARGUMENT, "ns_rotary: rows or heads of the output overlap");
     NS_REQUIRE(x != y || (x_ld == y_ld && x_head == y_head), NS_ERR_ARGUMENT, "ns_rotary: in place, both pitches have to be the input's");
     NsDevice* d = ns_dev(h);
@@ -354,7 +468,7 @@ extern "C" int ns_rotary(ns_device_t h, uint64_t x, int dtype, int64_t x_ld, int
     if (rows == 0) return NS_OK;
     RotaryArgs p;
     p.x = reinterpret_cast<const void*>(x); p.y = reinterpret_cast<void*>(y);
-    p.x_ld = x_ld; p.x_head = x_head; p.y_ld = y_ld; p.y_head = y_head;
+    p.x_ld = (int)x_ld; p.x_head = (int)x_head; p.y_ld = (int)y_ld; p.y_head = (int)y_head;
     p.pos = reinterpret_cast<const int32_t*>(pos);
     p.freq = reinterpret_cast<const float*>(freq);
     p.amplitude = amplitude; p.sign = inverse ? -1.0f : 1.0f;
@@ -365,17 +479,19 @@ extern "C" int ns_rotary(ns_device_t h, uint64_t x, int dtype, int64_t x_ld, int
     return rot_pick(halves, vec, [&](auto hv, auto vc) {
         constexpr bool HALVES = decltype(hv)::value;
         constexpr int VEC = decltype(vc)::value;
-        const RotTasks<HALVES, VEC> n(dim, rot_dims, p.copies != 0);
-        p.group = rot_group((int64_t)heads * n.per_head);
-        const int per_cta = ROT_THREADS / p.group;
+        const RotTasks<HALVES, VEC> n(dim, rot_dims);
         // few rows: their heads are spread over CTAs, a task a thread at least
-        int64_t ctas = (rows + per_cta - 1) / per_cta;
         int parts = 1;
-        while (parts < heads && ctas * parts < d->sm_count && (int64_t)heads * n.per_head > (int64_t)parts * ROT_THREADS) parts *= 2;
+        while (parts < heads && rows * parts < d->sm_count && (int64_t)heads * n.turned > (int64_t)parts * ROT_THREADS) parts *= 2;
         p.heads_each = (heads + parts - 1) / parts;
         parts = (heads + p.heads_each - 1) / p.heads_each;
+        p.lanes = rot_lanes(d, rows, p.heads_each, n.turned, n.table(), p.heads_each * dim);
+        p.half = RotDiv(rot_dims / 2);
+        p.rest = RotDiv((dim - n.rest) / VEC);
+        p.rest_row = RotDiv(heads * ((dim - n.rest) / VEC));       // (several rows a CTA: parts is 1)
+        int64_t ctas = (rows + p.lanes.rows - 1) / p.lanes.rows;
         if (ctas > (1 << 30)) ctas = 1 << 30;
-        const size_t smem = (size_t)per_cta * (rot_dims / 2) * sizeof(float2);
+        const size_t smem = (size_t)p.lanes.rows * n.table() * sizeof(float2);
         const dim3 grid((unsigned)ctas, (unsigned)parts);
         if constexpr (VEC <= 4) {
             if (size == 4) {
@@ -403,7 +519,7 @@ extern "C" int ns_kv_append_rotary(ns_device_t h, ns_kv_cache_t cache, uint64_t 
     const int dim = c.head_dim;
     NS_REQUIRE(rot_dims >= 2 && rot_dims <= dim && rot_dims % 2 == 0, NS_ERR_ARGUMENT, "ns_kv_append_rotary: rot_dims must be even, 2 to %d (got %d)", dim, rot_dims);
     if (q == 0) heads = 0;
-    NS_REQUIRE((int64_t)(heads + 2LL * c.heads) * dim <= (1 << 24), NS_ERR_ARGUMENT, "ns_kv_append_rotary: at most 2^24 columns a row");
+    NS_REQUIRE((int64_t)(heads + 2LL * c.heads) * dim <= ROT_MAX_COLUMNS, NS_ERR_ARGUMENT, "ns_kv_append_rotary: at most 2^19 columns a row");
     NS_REQUIRE(k_col >= 0 && v_col >= 0 && (q == 0 || q_col >= 0) && (int64_t)k_col + c.heads * dim <= src_ld && (int64_t)v_col + c.heads * dim <= src_ld &&
                    (q == 0 || (int64_t)q_col + heads * dim <= src_ld),
                NS_ERR_ARGUMENT, "ns_kv_append_rotary: columns outside the source's rows");
@@ -439,20 +555,22 @@ extern "C" int ns_kv_append_rotary(ns_device_t h, ns_kv_cache_t cache, uint64_t 
     return rot_pick(halves, vec, [&](auto hv, auto vc) {
         constexpr bool HALVES = decltype(hv)::value;
         constexpr int VEC = decltype(vc)::value;
-        const RotTasks<HALVES, VEC> n(dim, rot_dims, true);
-        const int tasks = (heads + c.heads) * n.per_head + c.heads * (dim / VEC);
-        p.group = rot_group(tasks);
-        const int per_cta = ROT_THREADS / p.group;
-        const int ctas = (rows + per_cta - 1) / per_cta;
-        int parts = 1;
-        while (ctas * parts < 2 * d->sm_count && tasks > parts * ROT_THREADS) parts *= 2;
-        p.tasks_each = (tasks + parts - 1) / parts;
-        parts = (tasks + p.tasks_each - 1) / p.tasks_each;
-        const size_t smem = (size_t)per_cta * (rot_dims / 2) * sizeof(float2);
-        const dim3 grid((unsigned)ctas, (unsigned)parts);
-        return ns_pick_slabs<NS_IN_TURN>(splits > 2 && rows <= 128, [&](auto sl) {
-            NS_CUDA(ns_launch_plain(ns_kv_append_rotary_kernel<HALVES, VEC, decltype(sl)::value>, grid, dim3(ROT_THREADS), smem, d->stream, p));
+        const RotTasks<HALVES, VEC> n(dim, rot_dims);
+        p.lane_tasks = n.turned < 32 ? n.turned : 32;
+        // few rows: until there are eight warps an SM, or each has one turn
+        const int turns = (heads + c.heads + 32 / p.lane_tasks - 1) / (32 / p.lane_tasks);
+        p.parts = 1;
+        while ((int64_t)rows * p.parts < 8 * d->sm_count && p.parts < turns) p.parts *= 2;
+        p.rest = RotDiv((dim - n.rest) / VEC);
+        p.value = RotDiv(dim / VEC);
+        const int64_t items = (int64_t)rows * p.parts;
+        const size_t smem = (size_t)(ROT_THREADS / 32) * n.table() * sizeof(float2);
+        const dim3 grid((unsigned)((items + ROT_THREADS / 32 - 1) / (ROT_THREADS / 32)));
+        auto launch = [&](auto kernel) {
+            NS_CUDA(ns_launch_plain(kernel, grid, dim3(ROT_THREADS), smem, d->stream, p));
             return (int)NS_OK;
-        });
+        };
+        if (src_dtype == NS_BF16) return launch(ns_kv_append_rotary_kernel<HALVES, VEC, ROT_BF16>);
+        return ns_pick_slabs<NS_IN_TURN>(splits > 2 && rows <= 128, [&](auto sl) { return launch(ns_kv_append_rotary_kernel<HALVES, VEC, decltype(sl)::value>); });
     });
 }

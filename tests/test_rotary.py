@@ -189,6 +189,8 @@ def test_rotary_refusals():
     call("overlap", y=2 * A, y_ld=255)
     call("overlap", y=2 * A, y_ld=128, y_head=128)
     call("negative pitch", x_ld=-256)
+    call("2^31", x_ld=1 << 31)
+    call("2^19 columns", heads=8192, x_head=0, y=2 * A, y_head=128, y_ld=1 << 20)
     call("device handle is null", y=2 * A, y_ld=128, y_head=512)      # rows inside heads
     call("device handle is null", y=2 * A, x_ld=0)                    # one row for all
 
