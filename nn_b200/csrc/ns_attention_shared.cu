@@ -11,7 +11,7 @@
 // r % group of its group.
 #include <math.h>
 
-#include "ns_cache.cuh"
+#include "ns_attention_shared.cuh"
 #include "ns_mma.cuh"
 
 namespace {
@@ -21,42 +21,12 @@ constexpr int SH_THREADS = 32 * SH_WARPS;
 constexpr int SH_KEYS = 16;                // keys a warp takes at a time
 constexpr int SH_ROWS = 16;                // query rows of a CTA
 constexpr int SH_STAGES = 3;
-constexpr int SH_BAD_PAGE = 520;           // status: a page-table entry that names no page of the pool
-
-struct SharedParams {
-    const uint16_t* q;
-    int64_t q_stride;
-    uint16_t* o;
-    int64_t o_stride;
-    const uint16_t* k_pool;
-    const uint16_t* v_pool;
-    const int32_t* prefix_table;
-    const int32_t* prefix_len;
-    const int32_t* page_table;
-    const int32_t* pos;
-    const int32_t* lens;
-    int prefix_pages, max_pages, page_shift, num_pages;
-    int batch, steps, heads, kv_heads, group;
-    int prefix_tiles, prefix_splits;       // row tiles over all sequences, parts by position
-    int own_tiles, own_splits;
-    float scale_log2;
-    float* part_o;                         // [parts, kv_heads, rows, head_dim]
-    float2* part_ml;                       // [parts, kv_heads, rows]: maximum in units of log2, sum
-    int* status;
-};
 
 // 16 bytes to shared memory, zeros where there is nothing
 __device__ __forceinline__ void sh_copy16(uint32_t dst, const void* src, bool there)
 {
     const int n = there ? 16 : 0;
     asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(dst), "l"(src), "r"(n) : "memory");
-}
-
-// How many positions a part's table can name, and of them how many count.
-__device__ __forceinline__ int sh_clamp(int64_t n, int pages, int shift)
-{
-    const int64_t most = (int64_t)pages << shift;
-    return (int)(n < 0 ? 0 : n < most ? n : most);
 }
 
 // A CTA: 16 rows of one key/value head against a range of keys.  Each warp walks 16 keys at a time on its own, through a ring of its own in shared memory, with
@@ -78,10 +48,10 @@ __global__ void __launch_bounds__(SH_THREADS) ns_attention_shared_walk_kernel(co
 
     // ---- which rows and which keys
     int item = blockIdx.x;
-    const int n_prefix = p.kv_heads * p.prefix_tiles * p.prefix_splits;
+    const int n_prefix = p.kv_heads * p.prefix_tiles * p.prefix_parts;
     const bool prefix = item < n_prefix;
     if (!prefix) item -= n_prefix;
-    const int splits = prefix ? p.prefix_splits : p.own_splits, tiles = prefix ? p.prefix_tiles : p.own_tiles;
+    const int splits = prefix ? p.prefix_parts : p.own_parts, tiles = prefix ? p.prefix_tiles : p.own_tiles;
     const int split = item % splits; item /= splits;
     const int tile = item % tiles; item /= tiles;
     const int kvh = item % p.kv_heads, b = item / p.kv_heads;       // b: 0 for the prefix
@@ -89,7 +59,7 @@ __global__ void __launch_bounds__(SH_THREADS) ns_attention_shared_walk_kernel(co
     const int seq_rows = p.steps * p.group;
     const int row0 = (prefix ? 0 : b * seq_rows) + tile * SH_ROWS;
     const int row_end = prefix ? rows_all : (b + 1) * seq_rows;
-    const int part = prefix ? split : p.prefix_splits + split;
+    const int part = prefix ? split : p.prefix_parts + split;
     const int32_t* table = prefix ? p.prefix_table : p.page_table + (int64_t)b * p.max_pages;
     const int table_pages = prefix ? p.prefix_pages : p.max_pages;
     // own positions: how many the token of row r sees
@@ -257,7 +227,7 @@ __global__ void __launch_bounds__(SH_THREADS) ns_attention_shared_walk_kernel(co
         for (int h = 0; h < 2; h++)
             *reinterpret_cast<float2*>(out + (fr + 8 * h) * (DH + 4) + n * 8 + fc) = make_float2(acc[n][2 * h], acc[n][2 * h + 1]);
     __syncthreads();
-    const bool alone = p.prefix_splits + p.own_splits == 1;
+    const bool alone = p.part_o == nullptr;
     for (int e = threadIdx.x; e < SH_ROWS * DH; e += SH_THREADS) {
         const int rr = e / DH, c = e % DH, r = row0 + rr;
         if (r >= row_end) break;
@@ -291,7 +261,7 @@ __global__ void __launch_bounds__(256) ns_attention_shared_fold_kernel(const Sha
     constexpr int N = DH / 32;
     ns_pdl_wait();
     ns_pdl_trigger();
-    const int rows_all = p.batch * p.steps * p.group, parts = p.prefix_splits + p.own_splits;
+    const int rows_all = p.batch * p.steps * p.group, parts = p.prefix_parts + p.own_parts;
     const int64_t idx = (int64_t)blockIdx.x * 8 + (threadIdx.x >> 5);
     const int lane = threadIdx.x & 31;
     if (idx >= (int64_t)p.kv_heads * rows_all) return;
@@ -309,7 +279,8 @@ __global__ void __launch_bounds__(256) ns_attention_shared_fold_kernel(const Sha
 #pragma unroll 4
     for (int k = 0; k < parts; k++) {
         const float2 ml = p.part_ml[idx + k * step];
-        const float f = ml.x == -INFINITY ? (ml.y == 0.0f ? 0.0f : 1.0f) : ns_exp2(ml.x - M);
+        if (ml.x == -INFINITY && ml.y == 0.0f) continue;       // (its values were not written)
+        const float f = ml.x == -INFINITY ? 1.0f : ns_exp2(ml.x - M);
         L = fmaf(ml.y, f, L);
         const float* src = p.part_o + (idx + k * step) * DH + lane * N;
 #pragma unroll
@@ -326,12 +297,14 @@ int launch_shared(NsDevice* d, const SharedParams& p)
 {
     constexpr int smem = SH_WARPS * SH_STAGES * 2 * SH_KEYS * (DH + 8) * 2;
     static_assert(smem >= SH_WARPS * SH_ROWS * (DH + 4) * 4, "the fold's rows");
-    const int64_t ctas = (int64_t)p.kv_heads * ((int64_t)p.prefix_tiles * p.prefix_splits + (int64_t)p.batch * p.own_tiles * p.own_splits);
+    const int64_t ctas = (int64_t)p.kv_heads * ((int64_t)p.prefix_tiles * p.prefix_parts + (int64_t)p.batch * p.own_tiles * p.own_parts);
     NS_REQUIRE(ctas < (1LL << 31), NS_ERR_ARGUMENT, "ns_attention_shared: too many rows");
-    auto walk = ns_attention_shared_walk_kernel<DH>;
-    NS_CUDA(cudaFuncSetAttribute(walk, cudaFuncAttributeMaxDynamicSharedMemorySize, smem));
-    NS_CUDA(ns_launch_plain(walk, dim3((unsigned)ctas), dim3(SH_THREADS), smem, d->stream, p));
-    if (p.prefix_splits + p.own_splits > 1) {
+    if (ctas > 0) {
+        auto walk = ns_attention_shared_walk_kernel<DH>;
+        NS_CUDA(cudaFuncSetAttribute(walk, cudaFuncAttributeMaxDynamicSharedMemorySize, smem));
+        NS_CUDA(ns_launch_plain(walk, dim3((unsigned)ctas), dim3(SH_THREADS), smem, d->stream, p));
+    }
+    if (p.part_o != nullptr) {
         const int64_t rows = (int64_t)p.batch * p.steps * p.heads;
         NS_CUDA(ns_launch_plain(ns_attention_shared_fold_kernel<DH>, dim3((unsigned)((rows + 7) / 8)), dim3(256), 0, d->stream, p));
     }
@@ -386,20 +359,28 @@ extern "C" int ns_attention_shared(ns_device_t h, ns_kv_cache_t cache, uint64_t 
         if (n > (positions + 63) / 64) n = (positions + 63) / 64;
         return (int)(n < 1 ? 1 : n > 64 ? 64 : n);
     };
-    p.prefix_tiles = (int)((rows + SH_ROWS - 1) / SH_ROWS);
-    p.prefix_splits = prefix_pages == 0 ? 0 : parts((int64_t)p.prefix_tiles * c.heads, (int64_t)prefix_pages * c.page_size);
+    p.prefix_tiles = 0;
+    const bool tiles = ns_attention_shared_tiles_fit(d, p, c.head_dim, scale, &p.prefix_parts);
+    if (!tiles) {
+        p.prefix_tiles = (int)((rows + SH_ROWS - 1) / SH_ROWS);
+        p.prefix_parts = prefix_pages == 0 ? 0 : parts((int64_t)p.prefix_tiles * c.heads, (int64_t)prefix_pages * c.page_size);
+    }
     p.own_tiles = (steps * p.group + SH_ROWS - 1) / SH_ROWS;
-    p.own_splits = max_pages == 0 ? 0 : parts((int64_t)batch * p.own_tiles * c.heads, (int64_t)max_pages * c.page_size);
-    const int n_parts = p.prefix_splits + p.own_splits;
+    p.own_parts = max_pages == 0 ? 0 : parts((int64_t)batch * p.own_tiles * c.heads, (int64_t)max_pages * c.page_size);
+    const int n_parts = p.prefix_parts + p.own_parts;
     p.part_o = nullptr;
     p.part_ml = nullptr;
-    if (n_parts > 1) {
+    if (tiles || n_parts > 1) {
         const size_t sums = (size_t)n_parts * c.heads * rows;
         void* s = nullptr;
         rc = ns_scratch_reserve(d, sums * (c.head_dim * 4 + 8), &s);
         if (rc != NS_OK) return rc;
         p.part_o = reinterpret_cast<float*>(s);
         p.part_ml = reinterpret_cast<float2*>(p.part_o + sums * c.head_dim);
+    }
+    if (tiles) {
+        rc = ns_attention_shared_tiles(d, p, c.head_dim);
+        if (rc != NS_OK) return rc;
     }
     switch (c.head_dim) {
         case 32: return launch_shared<32>(d, p);
