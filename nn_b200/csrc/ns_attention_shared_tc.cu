@@ -1,13 +1,16 @@
 // The shared prefix of ns_attention_shared on the sm_100a tensor cores: the query rows of all sequences against each key/value head's pages, S = Q.K^T and
 // O += P.V as tcgen05.mma with accumulators in tensor memory, an online softmax between them.
 //
-// A tile is 256 query rows of one key/value head against a range of key blocks of 128; 384 threads, one persistent CTA per SM:
+// A tile is 256 query rows of one key/value head, its units the key blocks of 128; the units of all tiles, one after the other, are dealt out to the CTAs in equal
+// shares, one persistent CTA of 384 threads per SM.  What a CTA has of a tile is a part of its rows' results.
 //   warp 0       reads the page table and loads K and V blocks (a TMA box a page, or part of one) into rings of slots, for both groups
-//   warps 1, 2   issue the MMAs of group 0 and of group 1: O += P.V of a block, then S = Q.K^T of the next
+//   warp 1       issues the MMAs, in turn for group 0 and group 1: O += P.V of a block, then S = Q.K^T of the next
 //   warps 4..11  two groups of four warps; thread r of a group owns one query row (tensor-memory lane r): it copies its query to shared memory, and for each
 //                block reads 128 scores, takes maximum and sum, and writes P as bf16 over the scores in tensor memory, from where P.V takes it
 // Group g owns rows [128 g, 128 g + 128) of the tile and both groups read every block; with 128 rows or fewer they own the same rows and take turns
-// with the blocks, each a part of its own.  A group's softmax runs while the other's MMAs do.
+// with the blocks, each a part of its own.
+// One warp issues for both groups so that their MMAs run in that order.  With a warp for each the tensor pipe took them alternately, both groups' scores
+// arrived together, both computed exponentials together (3 300 cycles a block for 1 700 alone) and both then waited 1 200 cycles for MMAs.
 //
 // A block's positions behind the prefix's end are masked, and their values, which may be anything, are zeroed in shared memory before the MMA reads them (0 times NaN
 // is NaN); pages outside the pool read as zeros and are masked.  Parts leave as 32-bit sums; ns_attention_shared_fold_kernel joins them.
@@ -42,30 +45,51 @@ struct Layout {
 struct TileParams {
     SharedParams s;
     int rows;            // query rows of a key/value head
-    int tiles, splits;   // row tiles, ranges of key blocks
+    int tiles;           // row tiles of a key/value head
     int turns;           // the groups own the same rows and take turns with the blocks
     int box;             // rows of a TMA box: a page, or 128 of it
+    int parts;           // of a tile, at most (each two where the groups take turns)
 };
 struct TileMaps {
     CUtensorMap k, v;    // [64 columns, box rows] of (columns, page rows, heads, pages)
     CUtensorMap o;       // [32 columns, 32 rows] of (columns, rows, parts * heads), float
 };
 
+// What a CTA has of a tile: key blocks [b0, b1), and which part of the tile that is.
 struct Item {
-    int kvh, tile, split, b0, b1;      // key blocks [b0, b1)
+    int kvh, tile, part, b0, b1;
 };
-__device__ __forceinline__ Item tile_item(const TileParams& p, int idx, int n_keys)
-{
-    Item t;
-    // neighbours read the same keys
-    t.tile = idx % p.tiles; idx /= p.tiles;
-    t.split = idx % p.splits;
-    t.kvh = idx / p.splits;
-    const int64_t blocks = (n_keys + ST_KB - 1) / ST_KB;
-    t.b0 = (int)(blocks * t.split / p.splits);
-    t.b1 = (int)(blocks * (t.split + 1) / p.splits);
-    return t;
-}
+// The CTAs' shares: units [first, end) of all, walked item by item.
+struct Share {
+    int blocks;          // of a tile
+    int64_t at, end, total;
+    int ctas;
+    __device__ __forceinline__ Share(const TileParams& p, int n_keys)
+    {
+        blocks = (n_keys + ST_KB - 1) / ST_KB;
+        total = (int64_t)blocks * p.tiles * p.s.kv_heads;
+        ctas = (int)(total < gridDim.x ? total : gridDim.x);       // no share is empty but behind these
+        at = end = 0;
+        if ((int)blockIdx.x < ctas) {
+            at = total * blockIdx.x / ctas;
+            end = total * (blockIdx.x + 1) / ctas;
+        }
+    }
+    __device__ __forceinline__ bool next(const TileParams& p, Item& t)
+    {
+        if (at >= end) return false;
+        const int tile = (int)(at / blocks);
+        const int64_t first = (int64_t)tile * blocks;
+        t.kvh = tile / p.tiles;
+        t.tile = tile - t.kvh * p.tiles;
+        t.b0 = (int)(at - first);
+        t.b1 = (int)(end - first < blocks ? end - first : blocks);
+        // the CTA that has a unit x is the last one whose share begins at or before it
+        t.part = (int)blockIdx.x - (int)(((first + 1) * ctas - 1) / total);
+        at = first + t.b1;
+        return true;
+    }
+};
 
 __device__ __forceinline__ float st_exp2(float x)
 {
@@ -162,7 +186,6 @@ __global__ void __launch_bounds__(ST_THREADS, 1) ns_attention_shared_tile_kernel
     auto bar = [&](int i) { return bar_base + 8u * i; };
     const uint32_t tmem_slot = bar(L::COUNT);
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-    const int items = p.s.kv_heads * p.splits * p.tiles;
 
     if (threadIdx.x == 0) {
         abort_flag_storage = 0;
@@ -173,9 +196,9 @@ __global__ void __launch_bounds__(ST_THREADS, 1) ns_attention_shared_tile_kernel
         }
         for (int i = 0; i < L::SLOTS; i++) {
             ns_mbar_init(bar(L::K_FULL + i), 1);
-            ns_mbar_init(bar(L::K_EMPTY + i), 2);
+            ns_mbar_init(bar(L::K_EMPTY + i), 1);
             ns_mbar_init(bar(L::V_FULL + i), 1);
-            ns_mbar_init(bar(L::V_EMPTY + i), 2);
+            ns_mbar_init(bar(L::V_EMPTY + i), 1);
         }
         for (int i = 0; i < 4; i++) ns_mbar_init(bar(L::P_FULL + i), 4);
         ns_mbar_init(bar(L::V_TAIL), 1);
@@ -200,9 +223,10 @@ __global__ void __launch_bounds__(ST_THREADS, 1) ns_attention_shared_tile_kernel
     const int n_keys = sh_clamp(p.s.prefix_len[0], p.s.prefix_pages, p.s.page_shift);
     const int code = 330;
     auto wait = [&](int i, uint32_t parity, int what) { return ns_mbar_wait_warp(bar(i), parity & 1u, abort_flag, p.s.status, code + what); };
-    // whether group g has rows in a tile, and whether it takes block j of an item
+    // whether group g has rows in a tile
     auto has_rows = [&](int g, const Item& t) { return p.turns != 0 || t.tile * 256 + 128 * g < p.rows; };
-    auto takes = [&](int g, const Item& t, int j) { return p.turns == 0 || ((j - t.b0) & 1) == g; };
+    Share share(p, n_keys);
+    Item t;
     // the page of box `lane` of a block: -1 behind the prefix
     const int boxes = ST_KB / p.box, shift = p.s.page_shift;
     auto box_page = [&](int j) {
@@ -220,8 +244,7 @@ __global__ void __launch_bounds__(ST_THREADS, 1) ns_attention_shared_tile_kernel
             Ring<L::SLOTS> ring;
             uint32_t tails = 0;
             bool ok = true;
-            for (int idx = blockIdx.x; ok && idx < items; idx += gridDim.x) {
-                const Item t = tile_item(p, idx, n_keys);
+            while (ok && share.next(p, t)) {
                 int page = t.b0 < t.b1 ? box_page(t.b0) : -1;
                 for (int j = t.b0; j < t.b1; j++, ring.next()) {
                     const int next = j + 1 < t.b1 ? box_page(j + 1) : -1;
@@ -264,88 +287,68 @@ __global__ void __launch_bounds__(ST_THREADS, 1) ns_attention_shared_tile_kernel
                     page = next;
                 }
             }
-        } else if (warp < 3) {
-            // ------------------------------------------------------------ MMAs of one group
-            const int g = warp - 1;
+        } else if (warp == 1) {
+            // ------------------------------------------------------------ MMAs
             const bool leader = ns_elect();
             constexpr uint32_t idesc_qk = ns_idesc(1, 1, 0, 0, 128, ST_KB), idesc_pv = ns_idesc(1, 1, 0, 1, 128, DH);
             const uint64_t desc_k = ns_desc_base(16, 1024);
             const uint64_t desc_v = ns_desc_base(L::HALF, 1024);      // MN-major: the halves of 64 columns, 8 key rows 1 KB apart
-            const uint32_t o_tmem = tmem_base + 256 * g, s_tmem = o_tmem + ST_S_COL, q_smem = smem_base + L::Q * g;
             Ring<L::SLOTS> kr, vr;
-            uint32_t nq = 0, kp = 0;      // items and blocks so far
+            uint32_t nq[2] = {0, 0}, kp[2] = {0, 0};                  // of each group: items and blocks so far
             bool ok = true;
-            // blocks that are the other group's are given back when they have arrived (an earlier arrival would count for the block before them in
-            // the slot)
-            auto skip_k = [&]() {
-                ok = ok && wait(L::K_FULL + kr.s, kr.phase, 4);
-                if (ok && leader) ns_mbar_arrive(bar(L::K_EMPTY + kr.s));
-                kr.next();
-            };
-            auto skip_v = [&]() {
-                ok = ok && wait(L::V_FULL + vr.s, vr.phase, 5);
-                if (ok && leader) ns_mbar_arrive(bar(L::V_EMPTY + vr.s));
-                vr.next();
-            };
-            auto scores = [&]() {
-                ok = ok && wait(L::K_FULL + kr.s, kr.phase, 4);
-                if (!ok) return;
+            // the scores of group g for the block in the key ring's slot; `free`: the last ones that need it
+            auto scores = [&](int g, bool free) {
                 ns_tc_fence_after();
                 if (leader) {
-                    const uint32_t kb = smem_base + L::K_AT + kr.s * L::KV;
+                    const uint32_t kb = smem_base + L::K_AT + kr.s * L::KV, qb = smem_base + L::Q * g, s_tmem = tmem_base + 256 * g + ST_S_COL;
 #pragma unroll
                     for (int kk = 0; kk < DH / 16; kk++)
-                        ns_mma_f16(s_tmem, ns_desc_at(desc_k, q_smem + (kk >> 2) * (128 * 128) + (kk & 3) * 32),
+                        ns_mma_f16(s_tmem, ns_desc_at(desc_k, qb + (kk >> 2) * (128 * 128) + (kk & 3) * 32),
                                    ns_desc_at(desc_k, kb + (kk >> 2) * L::HALF + (kk & 3) * 32), idesc_qk, kk > 0 ? 1u : 0u);
                     ns_tc_commit(bar(L::S_FULL + g));
-                    ns_tc_commit(bar(L::K_EMPTY + kr.s));
+                    if (free) ns_tc_commit(bar(L::K_EMPTY + kr.s));
                 }
-                kr.next();
+                if (free) kr.next();
             };
-            for (int idx = blockIdx.x; ok && idx < items; idx += gridDim.x) {
-                const Item t = tile_item(p, idx, n_keys);
-                const bool mine = has_rows(g, t);
-                int first = t.b0;
-                while (first < t.b1 && !(mine && takes(g, t, first))) first++;
-                // (a ring holds two blocks: its values are never left behind for keys further on)
-                if (first == t.b1) {
-                    for (int j = t.b0; j < t.b1 && ok; j++) {
-                        skip_k();
-                        skip_v();
-                    }
-                    continue;
+            while (ok && share.next(p, t)) {
+                const bool both = p.turns != 0 || has_rows(1, t);
+                const int step = p.turns ? 2 : 1;
+                // the first scores of each group: of one block, or of a block each
+                for (int g = 0; g < (both ? 2 : 1) && ok; g++) {
+                    if (p.turns && t.b0 + g >= t.b1) break;
+                    ok = wait(L::Q_FULL + g, nq[g]++, 6);
+                    if (ok && (g == 0 || p.turns)) ok = wait(L::K_FULL + kr.s, kr.phase, 4);
+                    if (ok) scores(g, p.turns || g == (both ? 1 : 0));
                 }
-                // K of the blocks before the first, and its scores; then V of each block in turn, the next scores behind its product
-                for (int j = t.b0; j < first && ok; j++) skip_k();
-                ok = ok && wait(L::Q_FULL + g, nq++, 6);
-                if (ok) scores();
-                bool started = false;
                 for (int j = t.b0; j < t.b1 && ok; j++) {
-                    if (!(mine && takes(g, t, j))) { skip_v(); continue; }
+                    const int g0 = p.turns ? (j - t.b0) & 1 : 0, g1 = p.turns ? g0 : both ? 1 : 0;
                     ok = wait(L::V_FULL + vr.s, vr.phase, 5);
+                    for (int g = g0; g <= g1 && ok; g++) {
+                        const uint32_t o_tmem = tmem_base + 256 * g, s_tmem = o_tmem + ST_S_COL;
 #pragma unroll
-                    for (int hf = 0; hf < 2; hf++) {
-                        ok = ok && wait(L::P_FULL + 2 * g + hf, kp, 7);
+                        for (int hf = 0; hf < 2; hf++) {
+                            ok = ok && wait(L::P_FULL + 2 * g + hf, kp[g], 7);
+                            if (!ok) break;
+                            ns_tc_fence_after();
+                            if (leader) {
+                                const uint32_t vb = smem_base + L::V_AT + vr.s * L::KV + hf * (64 * 128), pa = s_tmem + hf * 32;
+#pragma unroll
+                                for (int kk = 0; kk < 4; kk++)
+                                    st_mma_ts(o_tmem, pa + kk * 8, ns_desc_at(desc_v, vb + kk * (16 * 128)), idesc_pv, j - t.b0 >= step || hf > 0 || kk > 0 ? 1u : 0u);
+                            }
+                        }
                         if (!ok) break;
-                        ns_tc_fence_after();
+                        kp[g]++;
                         if (leader) {
-                            const uint32_t vb = smem_base + L::V_AT + vr.s * L::KV + hf * (64 * 128), pa = s_tmem + hf * 32;
-#pragma unroll
-                            for (int kk = 0; kk < 4; kk++)
-                                st_mma_ts(o_tmem, pa + kk * 8, ns_desc_at(desc_v, vb + kk * (16 * 128)), idesc_pv, started || hf > 0 || kk > 0 ? 1u : 0u);
+                            ns_tc_commit(bar(L::O_DONE + g));
+                            if (g == g1) ns_tc_commit(bar(L::V_EMPTY + vr.s));
+                        }
+                        if (j + step < t.b1) {
+                            if (g == g0) ok = wait(L::K_FULL + kr.s, kr.phase, 4);
+                            if (ok) scores(g, g == g1);
                         }
                     }
-                    if (!ok) break;
-                    started = true;
-                    kp++;
-                    if (leader) {
-                        ns_tc_commit(bar(L::O_DONE + g));
-                        ns_tc_commit(bar(L::V_EMPTY + vr.s));
-                    }
                     vr.next();
-                    int k = j + 1;
-                    for (; k < t.b1 && ok && !takes(g, t, k); k++) skip_k();
-                    if (k < t.b1 && ok) scores();
                 }
             }
         }
@@ -360,15 +363,24 @@ __global__ void __launch_bounds__(ST_THREADS, 1) ns_attention_shared_tile_kernel
         const float scale = p.s.scale_log2;
         uint32_t k = 0;                          // blocks of this group so far, over all items
         bool ok = true;
-        for (int idx = blockIdx.x; ok && idx < items; idx += gridDim.x) {
-            const Item t = tile_item(p, idx, n_keys);
+        // parts [part, end) of row `row` hold nothing
+        auto empty = [&](int part, int end, int kvh, int row) {
+            if (row < p.rows)
+                for (; part < end; part++) p.s.part_ml[((int64_t)part * p.s.kv_heads + kvh) * p.rows + row] = make_float2(-INFINITY, 0.0f);
+        };
+        const int turns = p.turns ? 2 : 1, parts = p.parts * turns;
+        if (share.total == 0)
+            for (int i = blockIdx.x; i < p.tiles * p.s.kv_heads; i += gridDim.x)
+                if (p.turns == 0 || g == 0) empty(0, parts, i / p.tiles, i % p.tiles * 256 + (p.turns ? 0 : 128 * g) + r);
+        while (ok && share.next(p, t)) {
             if (!has_rows(g, t)) continue;
             const int row = (p.turns ? 0 : t.tile * 256 + 128 * g) + r;
-            const int part = p.turns ? 2 * t.split + g : t.split;
-            const int64_t ml_at = ((int64_t)part * p.s.kv_heads + t.kvh) * p.rows + row;
-            const int step = p.turns ? 2 : 1, first = t.b0 + (p.turns ? g : 0);
+            const int part = t.part * turns + (p.turns ? g : 0);
+            const int step = turns, first = t.b0 + (p.turns ? g : 0);
+            // a tile's last part leaves the rest of them empty
+            if (t.b1 == share.blocks && (p.turns == 0 || g == 0)) empty((t.part + 1) * turns, parts, t.kvh, row);
             if (first >= t.b1) {
-                if (row < p.rows) p.s.part_ml[ml_at] = make_float2(-INFINITY, 0.0f);
+                empty(part, part + 1, t.kvh, row);
                 continue;
             }
             // the query: 16-byte piece c of row r at c ^ (r & 7).  (The group's scores before have all been computed: each warp has waited for the last.)
@@ -384,12 +396,16 @@ __global__ void __launch_bounds__(ST_THREADS, 1) ns_attention_shared_tile_kernel
                 __syncwarp();
                 if (lane == 0) ns_mbar_arrive(bar(L::Q_FULL + g));
             }
+            // whether a page of these blocks is none of the pool's
+            bool any_bad = false;
+            for (int key = t.b0 * ST_KB + lane * p.box; key < min(t.b1 * ST_KB, n_keys); key += 32 * p.box) {
+                const int page = p.s.prefix_table[key >> shift];
+                any_bad |= page < 0 || page >= p.s.num_pages;
+            }
+            any_bad = __any_sync(0xffffffffu, any_bad);
             float m_ref = -INFINITY;             // reference maximum (raw score units)
             float l_run = 0.0f;                  // sum of the exponentials relative to m_ref
-            int page = box_page(first);
             for (int j = first; j < t.b1; j += step, k++) {
-                const uint32_t bad = __ballot_sync(0xffffffffu, box_bad(j, page));
-                page = j + step < t.b1 ? box_page(j + step) : -1;
                 ok = wait(L::S_FULL + g, k, 11);
                 if (!ok) break;
                 ns_tc_fence_after();
@@ -413,7 +429,8 @@ __global__ void __launch_bounds__(ST_THREADS, 1) ns_attention_shared_tile_kernel
                     for (int c = 0; c < ST_KB; c++)
                         if (c >= live) s[c] = -INFINITY;
                 }
-                if (bad != 0) {
+                if (any_bad) {
+                    const uint32_t bad = __ballot_sync(0xffffffffu, box_bad(j, box_page(j)));
                     const int box_shift = 31 - __clz(p.box);
 #pragma unroll
                     for (int c = 0; c < ST_KB; c++)
@@ -466,7 +483,7 @@ __global__ void __launch_bounds__(ST_THREADS, 1) ns_attention_shared_tile_kernel
             ok = wait(L::O_DONE + g, k - 1, 12);
             if (!ok) break;
             ns_tc_fence_after();
-            if (row < p.rows) p.s.part_ml[ml_at] = make_float2(m_ref * scale, l_run);
+            if (row < p.rows) p.s.part_ml[((int64_t)part * p.s.kv_heads + t.kvh) * p.rows + row] = make_float2(m_ref * scale, l_run);
             // O -> shared memory (16-byte piece q of row r at q ^ (r & 7)) -> a TMA store a warp, 32 columns at a time; rows behind the last are clipped
             const int warp_row = row - lane;
 #pragma unroll 1
@@ -508,6 +525,24 @@ __global__ void __launch_bounds__(ST_THREADS, 1) ns_attention_shared_tile_kernel
     }
 }
 
+// CTAs, by the longest prefix: the SMs, or a unit each.
+int tile_ctas(const NsDevice* d, const TileParams& p)
+{
+    const int64_t blocks = (((int64_t)p.s.prefix_pages << p.s.page_shift) + ST_KB - 1) / ST_KB, units = blocks * p.tiles * p.s.kv_heads;
+    return (int)(units < d->sm_count ? units : d->sm_count);
+}
+
+void tile_plan(const NsDevice* d, const SharedParams& s, TileParams& p)
+{
+    p.s = s;
+    p.rows = s.batch * s.steps * s.group;
+    p.turns = p.rows <= 128 ? 1 : 0;
+    p.tiles = (p.rows + 255) / 256;
+    p.box = s.page_shift < 7 ? 1 << s.page_shift : ST_KB;
+    // a tile's units lie in the shares of at most one CTA more than fit into it, and one for a share that ends inside
+    p.parts = tile_ctas(d, p) / (p.tiles * s.kv_heads) + 2;
+}
+
 template <int DH>
 int launch_tiles(NsDevice* d, const TileParams& p)
 {
@@ -525,32 +560,11 @@ int launch_tiles(NsDevice* d, const TileParams& p)
     uint32_t o_box[3] = {32, 32, 1};
     rc = ns_make_tensor_map(&maps.o, CU_TENSOR_MAP_DATA_TYPE_FLOAT32, 3, p.s.part_o, o_dims, o_bytes, o_box, CU_TENSOR_MAP_SWIZZLE_128B);
     if (rc != NS_OK) return rc;
-    const int items = p.s.kv_heads * p.splits * p.tiles;
     auto kernel = ns_attention_shared_tile_kernel<DH>;
     NS_CUDA(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)L::SMEM));
-    kernel<<<items < d->sm_count ? items : d->sm_count, ST_THREADS, L::SMEM, d->stream>>>(maps, p);
+    kernel<<<tile_ctas(d, p), ST_THREADS, L::SMEM, d->stream>>>(maps, p);
     NS_CUDA(cudaGetLastError());
     return NS_OK;
-}
-
-// Row tiles and ranges of key blocks.  What a launch takes is its rounds over the SMs times an item's blocks and about four blocks' time for its
-// queries, first loads and results; every range also costs its results' way through memory.
-void tile_plan(const NsDevice* d, const SharedParams& s, TileParams& p)
-{
-    p.rows = s.batch * s.steps * s.group;
-    p.turns = p.rows <= 128 ? 1 : 0;
-    p.tiles = (p.rows + 255) / 256;
-    const int page = 1 << s.page_shift;
-    p.box = page < ST_KB ? page : ST_KB;
-    const int64_t blocks = ((int64_t)s.prefix_pages * page + ST_KB - 1) / ST_KB;
-    const int64_t tiles = (int64_t)p.tiles * s.kv_heads;
-    int64_t best = -1;
-    p.splits = 1;
-    for (int n = 1; n <= 64 && n <= blocks; n++) {
-        const int64_t rounds = (tiles * n + d->sm_count - 1) / d->sm_count, each = (blocks + n - 1) / n;
-        const int64_t cost = rounds * ((p.turns ? (each + 1) / 2 : each) + 4) * 8 + n;
-        if (best < 0 || cost < best) { best = cost; p.splits = n; }
-    }
 }
 
 }  // namespace
@@ -562,14 +576,13 @@ bool ns_attention_shared_tiles_fit(const NsDevice* d, const SharedParams& s, int
     if (head_dim < 64 || s.page_shift < 3 || !(scale > 0.0f) || s.prefix_pages == 0) return false;
     TileParams p;
     tile_plan(d, s, p);
-    *parts = p.splits * (p.turns ? 2 : 1);
+    *parts = p.parts * (p.turns ? 2 : 1);
     return true;
 }
 
 int ns_attention_shared_tiles(NsDevice* d, const SharedParams& s, int head_dim)
 {
     TileParams p;
-    p.s = s;
     tile_plan(d, s, p);
     return head_dim == 64 ? launch_tiles<64>(d, p) : launch_tiles<128>(d, p);
 }
