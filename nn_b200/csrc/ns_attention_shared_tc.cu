@@ -42,8 +42,20 @@ struct Layout {
     static_assert(SMEM <= 232448 && COUNT * 8 + 16 <= 512, "shared memory of an SM");
 };
 
+// n / d for n < 2^30: the multiplier is rounded up, which is exact there for every d (32 + log2 d bits of it)
+struct Divide {
+    uint32_t m, shift;
+    void by(int d)
+    {
+        shift = 0;
+        while ((1 << shift) < d) shift++;
+        m = (uint32_t)((((uint64_t)1 << (31 + shift)) + d - 1) / d);
+    }
+    __device__ __forceinline__ int of(int n) const { return (int)(((uint64_t)(uint32_t)n * m) >> (31 + shift)); }
+};
 struct TileParams {
     SharedParams s;
+    Divide group;
     int rows;            // query rows of a key/value head
     int tiles;           // row tiles of a key/value head
     int turns;           // the groups own the same rows and take turns with the blocks
@@ -137,13 +149,13 @@ __device__ __forceinline__ uint64_t st_fma2(uint64_t a, uint64_t b, uint64_t c)
     asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(y) : "l"(a), "l"(b), "l"(c));
     return y;
 }
-// P = 2^(s scale + neg_m) of 64 scores as pairs of bf16; the sums of P before that rounding go onto `sum`.
-template <int FIRST>
+// P = 2^(s scale + neg_m) of pairs [C0, C1) of the 64 scores from FIRST on, as bf16; the sums of P before that rounding go onto `sum`.
+template <int FIRST, int C0, int C1>
 __device__ __forceinline__ void st_exponentials(const float (&s)[ST_KB], float scale, float neg_m, uint64_t (&sum)[2], uint32_t (&pk)[32])
 {
     const uint64_t scale2 = st_pair(scale, scale), neg2 = st_pair(neg_m, neg_m);
 #pragma unroll
-    for (int c = 0; c < 32; c++) {
+    for (int c = C0; c < C1; c++) {
         float p0, p1;
         st_split(st_fma2(st_pair(s[FIRST + 2 * c], s[FIRST + 2 * c + 1]), scale2, neg2), p0, p1);
         p0 = st_exp2(p0);
@@ -243,7 +255,7 @@ __global__ void __launch_bounds__(ST_THREADS, 1) ns_attention_shared_tile_kernel
             const bool leader = ns_elect();
             Ring<L::SLOTS> ring;
             uint32_t tails = 0;
-            bool ok = true;
+            bool ok = true, begun = false;
             while (ok && share.next(p, t)) {
                 int page = t.b0 < t.b1 ? box_page(t.b0) : -1;
                 for (int j = t.b0; j < t.b1; j++, ring.next()) {
@@ -265,6 +277,13 @@ __global__ void __launch_bounds__(ST_THREADS, 1) ns_attention_shared_tile_kernel
                     ok = wait(L::K_EMPTY + ring.s, ring.phase ^ 1u, 1);
                     if (!ok) break;
                     load(&maps.k, smem_base + L::K_AT + ring.s * L::KV, bar(L::K_FULL + ring.s));
+                    // at the start 128 KB of keys and values an SM would stand in the queue to memory before the queries (3 us): only the first keys do
+                    if (!begun) {
+                        begun = true;
+                        ok = wait(L::Q_FULL, 0, 6);
+                        if (ok && (p.turns ? t.b0 + 1 < t.b1 : has_rows(1, t))) ok = wait(L::Q_FULL + 1, 0, 6);
+                        if (!ok) break;
+                    }
                     ok = wait(L::V_EMPTY + ring.s, ring.phase ^ 1u, 2);
                     if (!ok) break;
                     const uint32_t v = smem_base + L::V_AT + ring.s * L::KV;
@@ -383,24 +402,37 @@ __global__ void __launch_bounds__(ST_THREADS, 1) ns_attention_shared_tile_kernel
                 empty(part, part + 1, t.kvh, row);
                 continue;
             }
-            // the query: 16-byte piece c of row r at c ^ (r & 7).  (The group's scores before have all been computed: each warp has waited for the last.)
-            {
-                const int token = row / p.s.group;
-                const uint16_t* q = p.s.q + (int64_t)token * p.s.q_stride + (int64_t)(t.kvh * p.s.group + row - token * p.s.group) * DH;
-                uint4 w[DH / 8];
-#pragma unroll
-                for (int c = 0; c < DH / 8; c++) w[c] = row < p.rows ? *reinterpret_cast<const uint4*>(q + c * 8) : make_uint4(0, 0, 0, 0);
-#pragma unroll
-                for (int c = 0; c < DH / 8; c++) ns_st_shared_v4(q_smem + (c >> 3) * (128 * 128) + r * 128 + (((c & 7) ^ (r & 7)) * 16), w[c].x, w[c].y, w[c].z, w[c].w);
-                ns_fence_proxy_async();
-                __syncwarp();
-                if (lane == 0) ns_mbar_arrive(bar(L::Q_FULL + g));
-            }
-            // whether a page of these blocks is none of the pool's
+            // whether a page of these blocks is none of the pool's (the answers are awaited behind the queries)
             bool any_bad = false;
             for (int key = t.b0 * ST_KB + lane * p.box; key < min(t.b1 * ST_KB, n_keys); key += 32 * p.box) {
                 const int page = p.s.prefix_table[key >> shift];
                 any_bad |= page < 0 || page >= p.s.num_pages;
+            }
+            // the warp's 32 queries, whole rows side by side: 16-byte piece c of row r at c ^ (r & 7).  (The group's scores before have all been computed: each warp
+            // has waited for the last.)
+            {
+                constexpr int CH = DH / 8, PER = 32 / CH;             // pieces of a row, rows at a time
+                const int c = lane % CH, r0 = quad * 32 + lane / CH, base = row - r;
+                // (few instructions: this code is fetched cold, and unrolled with its divisions it took 7 000 cycles)
+                const int64_t head = (int64_t)t.kvh * p.s.group * DH + c * 8;
+#pragma unroll 1
+                for (int i = 0; i < 32; i += 8 * PER) {
+                    uint4 w[8];
+#pragma unroll
+                    for (int u = 0; u < 8; u++) {
+                        const int rr = base + r0 + i + u * PER, token = p.group.of(rr);
+                        w[u] = make_uint4(0, 0, 0, 0);
+                        if (rr < p.rows) w[u] = *reinterpret_cast<const uint4*>(p.s.q + head + (int64_t)token * p.s.q_stride + (rr - token * p.s.group) * DH);
+                    }
+#pragma unroll
+                    for (int u = 0; u < 8; u++) {
+                        const int rr = r0 + i + u * PER;
+                        ns_st_shared_v4(q_smem + (c >> 3) * (128 * 128) + rr * 128 + (((c & 7) ^ (rr & 7)) * 16), w[u].x, w[u].y, w[u].z, w[u].w);
+                    }
+                }
+                ns_fence_proxy_async();
+                __syncwarp();
+                if (lane == 0) ns_mbar_arrive(bar(L::Q_FULL + g));
             }
             any_bad = __any_sync(0xffffffffu, any_bad);
             float m_ref = -INFINITY;             // reference maximum (raw score units)
@@ -424,12 +456,12 @@ __global__ void __launch_bounds__(ST_THREADS, 1) ns_attention_shared_tile_kernel
                     }
                 }
                 const int live = n_keys - j * ST_KB;
-                if (live < ST_KB) {
+                if (__builtin_expect(live < ST_KB, 0)) {
 #pragma unroll
                     for (int c = 0; c < ST_KB; c++)
                         if (c >= live) s[c] = -INFINITY;
                 }
-                if (any_bad) {
+                if (__builtin_expect(any_bad, 0)) {
                     const uint32_t bad = __ballot_sync(0xffffffffu, box_bad(j, box_page(j)));
                     const int box_shift = 31 - __clz(p.box);
 #pragma unroll
@@ -447,7 +479,7 @@ __global__ void __launch_bounds__(ST_THREADS, 1) ns_attention_shared_tile_kernel
                     m_ref = mx;
                 }
                 // (these scores have followed the P.V before them through the tensor pipe: O is complete)
-                if (j > first && __any_sync(0xffffffffu, rescale)) {
+                if (__builtin_expect(j > first && __any_sync(0xffffffffu, rescale), 0)) {
 #pragma unroll 1
                     for (int c = 0; c < DH / 32; c++) {
                         uint32_t ob[32];
@@ -462,19 +494,22 @@ __global__ void __launch_bounds__(ST_THREADS, 1) ns_attention_shared_tile_kernel
                 // else nothing).
                 const float neg_m = m_ref == -INFINITY ? 0.0f : fmaf(m_ref, 0.0f, -m_ref * scale);
                 uint64_t sum[2] = {0, 0};
-                auto hand_over = [&](int hf, const uint32_t (&pk)[32]) {
-                    __syncwarp();
-                    ns_tmem_st32(s_addr + hf * 32, pk);
+                // P leaves for tensor memory half by half; the arrival of the first half is waited for inside the second's exponentials
+                auto handed = [&](int hf) {
                     ns_tc_wait_st();
                     ns_tc_fence_before();
                     __syncwarp();
                     if (lane == 0) ns_mbar_arrive(bar(L::P_FULL + 2 * g + hf));
                 };
-                uint32_t pk[32];
-                st_exponentials<0>(s, scale, neg_m, sum, pk);
-                hand_over(0, pk);
-                st_exponentials<64>(s, scale, neg_m, sum, pk);
-                hand_over(1, pk);
+                uint32_t pk[32], pk2[32];
+                st_exponentials<0, 0, 32>(s, scale, neg_m, sum, pk);
+                __syncwarp();
+                ns_tmem_st32(s_addr, pk);
+                st_exponentials<64, 0, 8>(s, scale, neg_m, sum, pk2);
+                handed(0);
+                st_exponentials<64, 8, 32>(s, scale, neg_m, sum, pk2);
+                ns_tmem_st32(s_addr + 32, pk2);
+                handed(1);
                 float l0, l1;
                 st_split(st_add2(sum[0], sum[1]), l0, l1);
                 l_run = l_run * alpha + (l0 + l1);
@@ -506,7 +541,7 @@ __global__ void __launch_bounds__(ST_THREADS, 1) ns_attention_shared_tile_kernel
             // the next item's first P.V overwrites O; it follows this warp's next P
             ns_tc_fence_before();
         }
-        if (lane == 0) ns_bulk_wait<0>();
+        if (lane == 0) ns_bulk_wait_read<0>();
     }
 
     // ---------------------------------------------------------------- teardown
@@ -536,6 +571,7 @@ void tile_plan(const NsDevice* d, const SharedParams& s, TileParams& p)
 {
     p.s = s;
     p.rows = s.batch * s.steps * s.group;
+    p.group.by(s.group);
     p.turns = p.rows <= 128 ? 1 : 0;
     p.tiles = (p.rows + 255) / 256;
     p.box = s.page_shift < 7 ? 1 << s.page_shift : ST_KB;
