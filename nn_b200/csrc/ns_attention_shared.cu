@@ -20,7 +20,7 @@ constexpr int SH_WARPS = 4;
 constexpr int SH_THREADS = 32 * SH_WARPS;
 constexpr int SH_KEYS = 16;                // keys a warp takes at a time
 constexpr int SH_ROWS = 16;                // query rows of a CTA
-constexpr int SH_STAGES = 3;
+constexpr int SH_STAGES = 2;
 
 // 16 bytes to shared memory, zeros where there is nothing
 __device__ __forceinline__ void sh_copy16(uint32_t dst, const void* src, bool there)
@@ -33,7 +33,7 @@ __device__ __forceinline__ void sh_copy16(uint32_t dst, const void* src, bool th
 // its own running maximum and sum; the four warps' results fold at the end.  P.V takes the weights as two bf16 halves: the rounding of
 // the output is then the only one that shows.
 template <int DH>
-__global__ void __launch_bounds__(SH_THREADS) ns_attention_shared_walk_kernel(const SharedParams p)
+__global__ void __launch_bounds__(SH_THREADS, 3) ns_attention_shared_walk_kernel(const SharedParams p)
 {
     constexpr int LD = DH + 8;                         // elements a row in shared memory: ldmatrix without conflicts
     constexpr int TILE = SH_KEYS * LD * 2;             // bytes

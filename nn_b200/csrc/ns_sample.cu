@@ -7,11 +7,14 @@
 // running sum of kept weights exceeds u times their sum.
 //
 // A draw is decided by whether a sum of up to 10^5 weights lies left or right of a border, so the weights are computed in 64 bits and summed as integers
-// of 2^-44: exact, whatever the order, the number of CTAs or the atomics.  (With 32-bit weights one row in a few thousand draws another token than the
+// of 2^-42: exact, whatever the order, the number of CTAs or the atomics.  (With 32-bit weights one row in a few thousand draws another token than the
 // definition's.)
 //
-// A cluster of 1 to 8 CTAs holds a row in shared memory; it is read from global memory once.  The cutoffs are found by histograms: first over
-// (max - x) / T in steps of 1/64, where weights down to 2^-44 spread over 2048 bins, then inside the bin over the bits of x, 11 at a time.
+// A cluster of 1 to 8 CTAs holds a row in shared memory; it is read from global memory once.  What remains costs passes over shared memory:
+//   - A top-k of up to ST_SORT_K: a histogram of every 16th token over (max - x) / T in steps of 1/64 names a cutoff that hardly ever fails to leave k candidates and leaves
+//     few more; they are gathered into one CTA, sorted (value, then index), cut by all three rules, sorted by index and drawn from.
+//   - Else cutoffs are found one after the other: the histogram of all tokens, by number or by weight, names the bin in which a cutoff lies, and that bin's tokens alone
+//     are gathered and sorted (or, where they are too many, counted by the bits of x, 11 at a time).  The draw is then one more pass over the row.
 #include <cooperative_groups.h>
 #include <math.h>
 
@@ -24,8 +27,12 @@ namespace {
 constexpr int ST_THREADS = 512;
 constexpr int ST_BINS = 2048;
 constexpr int ST_MAX_CLUSTER = 8;
-constexpr int ST_FIX = 44;                 // weights are multiples of 2^-44: 2^20 of them fit 64 bits
-constexpr int ST_TABLE = 128;              // 2^(-i / 128)
+constexpr int ST_FIX = 42;                 // weights are multiples of 2^-42: 2^20 of them fit 64 bits
+constexpr int ST_TABLE = 1024;             // 2^(-i / 1024)
+constexpr int ST_LIST = ST_THREADS;         // candidates that are sorted: one a thread
+constexpr int ST_SORT_K = 128;             // the largest top-k whose candidates they are
+constexpr int ST_SAMPLE = 16;              // its cutoff is guessed from every 16th token
+constexpr int ST_LIMB = 14;                // bits of a weight's share of a histogram's word: 2^18 of them fit
 constexpr uint32_t ST_NO_CUT = 0xFFFFFFFFu;
 
 struct SampleArgs {
@@ -41,28 +48,66 @@ struct SampleArgs {
     float* probs;
 };
 
+struct SampleTable {
+    uint64_t fixed[ST_TABLE];              // in units of 2^-42
+    float value[ST_TABLE];                 // the same as floats, times 2^42
+};
+
+// 2^42 * 2^(-i / 1024), rounded, made by the compiler from the series of e^x (64-bit exponentials would take every CTA microseconds).
+struct SamplePowers {
+    uint64_t v[ST_TABLE];
+    constexpr SamplePowers() : v()
+    {
+        for (int i = 0; i < ST_TABLE; i++) {
+            const double x = -0.69314718055994531 * i / ST_TABLE;
+            double sum = 0.0;
+            for (int k = 24; k > 0; k--) sum = (sum + 1.0) * x / k;
+            v[i] = (uint64_t)((sum + 1.0) * (double)(1ull << ST_FIX) + 0.5);
+        }
+    }
+};
+__device__ constexpr SamplePowers st_powers;
+
 struct SampleFound {
     int bin;
-    uint32_t count;                        // tokens of that bin
-    uint64_t before;                       // count or mass of the bins before it
+    uint64_t before;                       // number or weight of the bins before it
+};
+// Kept are the tokens whose (key, index) is not above `last`.
+struct SampleCut {
+    uint64_t last;
+    int bin;                               // its bin, where the run sums of gather() are to be used; -1: they are not
 };
 
 struct alignas(16) SampleShared {
-    uint32_t count[ST_BINS], lo[ST_BINS], hi[ST_BINS];
-    double table[ST_TABLE];
-    uint64_t part[ST_MAX_CLUSTER], mass[ST_MAX_CLUSTER], ties[ST_MAX_CLUSTER];       // of every CTA of the cluster; each written once or between barriers
+    union {
+        struct {
+            uint32_t word[3][ST_BINS];     // numbers, or weights in three shares of ST_LIMB bits
+        };
+        struct {
+            __align__(16) uint64_t list[ST_LIST];        // candidates: key, index
+            uint64_t sorted[ST_LIST], weights[ST_LIST];
+        };
+    };
+    int listed[ST_MAX_CLUSTER], mine;
+    SampleTable table;
+    uint64_t part[ST_MAX_CLUSTER], draw[ST_MAX_CLUSTER];       // of every CTA of the cluster, written between its barriers
+    uint64_t extra[ST_THREADS];            // of each thread's run
     uint64_t scan[ST_THREADS / 32], scan2[ST_THREADS / 32];
     float max[ST_MAX_CLUSTER];
     int max_at[ST_MAX_CLUSTER];
     float red[ST_THREADS / 32];
     int red_at[ST_THREADS / 32];
     SampleFound found;
+    uint64_t cut;
+    int run_first, run_end;
+    uint64_t run_before;
 };
 
-// not a number counts as -infinity, and both zeros are one value
+__device__ __forceinline__ float st_value(float x) { return x; }
+__device__ __forceinline__ float st_value(uint16_t x) { return ns_bf16_bits_to_f32(x); }
+// as a token is kept: what is no number counts as -infinity, and both zeros are one value
 __device__ __forceinline__ float st_clean(float x) { return x != x ? -INFINITY : x + 0.0f; }
-__device__ __forceinline__ float st_value(float x) { return st_clean(x); }
-__device__ __forceinline__ float st_value(uint16_t x) { return st_clean(ns_bf16_bits_to_f32(x)); }
+__device__ __forceinline__ uint16_t st_clean(uint16_t x) { return (x & 0x7FFF) > 0x7F80 ? 0xFF80 : x == 0x8000 ? 0 : x; }
 // ascending where the value descends
 __device__ __forceinline__ uint32_t st_key(float x)
 {
@@ -70,22 +115,52 @@ __device__ __forceinline__ uint32_t st_key(float x)
     return (b >> 31) ? b : ~b ^ 0x80000000u;
 }
 
-// e^(-d / T) in units of 2^-44, d = max - x >= 0.  z = 128 d / (T ln 2) = n + r; 2^(-z / 128) = 2^(-n / 128) times a polynomial of degree 4 in r (its next term is
-// below 2^-49); rounded to an integer once.  64-bit floats: d in 32 loses x's last bits, and z's fraction needs 44 of them.
+__device__ __forceinline__ float st_unkey(uint32_t key) { return __uint_as_float((key >> 31) ? key : ~key ^ 0x80000000u); }
+
+// the sum that a top-p asks for: the fewest units that are at least p times all of them, one at least
+__device__ __forceinline__ uint64_t st_goal(float p, uint64_t all)
+{
+    const uint64_t goal = p > 0.0f ? (uint64_t)ceil((double)p * (double)all) : 1;
+    return goal == 0 ? 1 : goal;
+}
+// A running sum exceeds u * total where it exceeds that number's floor.
+__device__ __forceinline__ uint64_t st_aim(float u, uint64_t total)
+{
+    const uint64_t aim = u < 1.0f ? (u > 0.0f ? (uint64_t)((double)u * (double)total) : 0) : total - 1;
+    return aim >= total ? total - 1 : aim;
+}
+
+// e^(-d / T) in units of 2^-42, d = max - x >= 0, within 2^-34 of itself (64-bit floats would take five times as long here: a warp's instruction 16 cycles).
+// d is a float and the rest of it, exactly; t = d / (T ln 2) the same to 2^-46 of itself; t = n + i / 1024 + r with |r| <= 2^-11;
+// 2^(-i / 1024) from a table, 2^(-r) = 1 + q with q a polynomial of degree 3 and below 2^-12, so that its float's error counts 2^-36; the product is rounded to an
+// integer once, and shifted by n.
 struct SampleWeight {
-    float max;
-    double rate;                           // 128 / (T ln 2)
-    const double* table;
+    float max, rate, rate_lo;              // 1 / (T ln 2): the float and the rest of it
+    const SampleTable* table;
+    __device__ __forceinline__ SampleWeight(float m, float temperature, const SampleTable* t) : max(m), table(t)
+    {
+        const double r = 1.4426950408889634 / (double)temperature;
+        rate = (float)fmin(r, 3e38);
+        rate_lo = (float)(fmin(r, 3e38) - (double)rate);
+    }
     __device__ __forceinline__ uint64_t operator()(float x) const
     {
-        if (x == max) return 1ull << ST_FIX;           // infinities among them
-        const double z = ((double)max - (double)x) * rate;
-        if (!(z < 128.0 * (ST_FIX + 2))) return 0;
-        const double n = rint(z), r = (z - n) * -0.0054152123481245726;        // -ln 2 / 128
-        const double e = fma(fma(fma(fma(r, 1.0 / 24, 1.0 / 6), r, 0.5), r, 1.0), r, 1.0);
-        const int i = (int)n;
-        const double w = e * table[i & (ST_TABLE - 1)];        // (1/2, 1], or an ulp above
-        return (uint64_t)__double2ll_rn(__longlong_as_double(__double_as_longlong(w) + ((long long)(ST_FIX - (i >> 7)) << 52)));
+        // both ends first: equal (infinities among them), and too far for half a unit
+        if (x == max) return 1ull << ST_FIX;
+        const float d = __fsub_rn(max, x);
+        const float p = __fmul_rn(d, rate);
+        if (!(p < (float)(ST_FIX + 2))) return 0;
+        // d + d_lo = max - x
+        const float back = __fsub_rn(d, max), d_lo = __fsub_rn(__fsub_rn(max, __fsub_rn(d, back)), __fadd_rn(x, back));
+        const float p_lo = fmaf(d_lo, rate, fmaf(d, rate_lo, fmaf(d, rate, -p)));
+        const float magic = 12582912.0f;   // 1.5 * 2^23: a sum's low bits are the rounded value
+        const float ni = fmaf(p, 1024.0f, magic);
+        const int steps = __float_as_int(ni) - __float_as_int(magic);          // n * 1024 + i
+        const float r = __fadd_rn(fmaf(__fsub_rn(ni, magic), -0.0009765625f, p), p_lo);        // (the product and its sum are exact)
+        const float q = r * fmaf(r, fmaf(r, -0.055504109f, 0.24022651f), -0.69314718f);        // 2^-r - 1
+        const int i = steps & (ST_TABLE - 1), n = steps >> 10;
+        const uint64_t w = table->fixed[i] + (int64_t)__float2int_rn(table->value[i] * q);
+        return n == 0 ? w : (w + (1ull << (n - 1))) >> n;
     }
 };
 
@@ -114,99 +189,280 @@ __device__ __forceinline__ uint64_t st_scan(uint64_t v, uint64_t* warps, uint64_
 
 __device__ __forceinline__ bool st_better(float v, int i, float w, int j) { return v > w || (v == w && i < j); }
 
+// the first histogram's bin: scale = 64 / T
+__device__ __forceinline__ int st_coarse(float x, float max, float scale)
+{
+    const float d = x == max ? 0.0f : max - x;
+    return __float_as_int(fminf(d * scale, (float)(ST_BINS - 1)) + 12582912.0f) - 0x4B400000;       // rounded by the sum with 1.5 * 2^23
+}
+
+// How many of `list`'s `count` values are below v (all different): every thread compares its own with all of them.
+__device__ __forceinline__ int st_rank(const uint64_t* list, int count, uint64_t v)
+{
+    int r = 0;
+    const ulonglong2* pairs = reinterpret_cast<const ulonglong2*>(list);
+#pragma unroll 4
+    for (int j = 0; j < count / 2; j++) {
+        const ulonglong2 w = pairs[j];
+        r += (w.x < v ? 1 : 0) + (w.y < v ? 1 : 0);
+    }
+    if ((count & 1) != 0) r += list[count - 1] < v ? 1 : 0;
+    return r;
+}
+
+struct SampleCuts {
+    int k;
+    float top_p, u;
+    uint64_t least;                        // smallest weight
+};
+
+// Draws from `count` candidates in s.list (key above, index below): by one CTA, the others have left.
+__device__ void st_draw(SampleShared& s, int count, const SampleCuts& cuts, const SampleWeight& weight, int row, const SampleArgs& p)
+{
+    const int tid = threadIdx.x;
+    if (tid < count) {
+        const uint64_t v = s.list[tid];
+        s.sorted[st_rank(s.list, count, v)] = v;
+    }
+    __syncthreads();
+    const uint64_t v = tid < count ? s.sorted[tid] : 0;
+    uint64_t w = tid < count && tid < cuts.k ? weight(st_unkey((uint32_t)(v >> 32))) : 0, total;
+    uint64_t before = st_scan(w, s.scan, total);
+    const uint64_t goal = cuts.top_p < 1.0f ? st_goal(cuts.top_p, total) : ~0ull;
+    // kept is the beginning; then by index
+    const int kept = __syncthreads_count(tid < count && tid < cuts.k && before < goal && w >= cuts.least);
+    if (tid < kept) s.list[tid] = v << 32 | (uint32_t)tid;
+    __syncthreads();
+    if (tid < kept) {
+        const uint64_t mine = v << 32 | (uint32_t)tid;
+        const int at = st_rank(s.list, kept, mine);
+        s.sorted[at] = mine >> 32;
+        s.weights[at] = w;
+    }
+    __syncthreads();
+    w = tid < kept ? s.weights[tid] : 0;
+    before = st_scan(w, s.scan2, total);
+    const uint64_t aim = st_aim(cuts.u, total);
+    if (before <= aim && aim < before + w) {
+        p.ids[row] = (int)s.sorted[tid];
+        if (p.probs != nullptr) p.probs[row] = (float)((double)w / (double)total);
+    }
+}
+
 template <typename T>
 struct SampleRow {
-    const SampleArgs& p;
+    static constexpr int VEC = 16 / sizeof(T);
     SampleShared& s;
-    const T* vals;                         // this CTA's tokens
-    int n, first;                          // how many, and the first's index
+    const T* vals;                         // this CTA's tokens; they begin `skew` after a vector
+    int n, first, skew;                    // how many, the first's index
     cg::cluster_group cl;
     int rank, ranks;
+    float max, scale;
 
-    // Clears the histogram, lets f(x) name each token's bin (negative: none) and adds it up, by weight too where `mass`.
+    // f(number in the CTA, value) for its tokens: vectors first, first + step .. below end
     template <typename F>
-    __device__ void histogram(bool mass, const SampleWeight& weight, F f)
+    __device__ __forceinline__ void each(int at, int step, int end, F f) const
     {
-        for (int i = threadIdx.x; i < ST_BINS; i += ST_THREADS) { s.count[i] = 0; s.lo[i] = 0; s.hi[i] = 0; }
-        __syncthreads();
-        for (int i = threadIdx.x; i < n; i += ST_THREADS) {
-            const float x = st_value(vals[i]);
-            const int bin = f(x);
-            if (bin < 0) continue;
-            atomicAdd(&s.count[bin], 1u);
-            if (mass) {
-                // a 64-bit sum in two words: the lower word's carry goes to the upper
-                const uint64_t w = weight(x);
-                const uint32_t lo = (uint32_t)w;
-                uint32_t hi = (uint32_t)(w >> 32);
-                if (lo != 0 && atomicAdd(&s.lo[bin], lo) + lo < lo) hi++;
-                if (hi != 0) atomicAdd(&s.hi[bin], hi);
+        const uint4* vecs = reinterpret_cast<const uint4*>(vals - skew);
+        for (int v = at; v < end; v += step) {
+            const uint4 raw = vecs[v];
+            const T* e = reinterpret_cast<const T*>(&raw);
+            const int i0 = v * VEC - skew;
+            if (i0 >= 0 && i0 + VEC <= n) {
+#pragma unroll
+                for (int i = 0; i < VEC; i++) f(i0 + i, st_value(e[i]));
+            } else {
+#pragma unroll
+                for (int i = 0; i < VEC; i++)
+                    if (i0 + i >= 0 && i0 + i < n) f(i0 + i, st_value(e[i]));
             }
         }
-        cl.sync();
     }
-    // The bin in which the sums over the cluster's histograms reach `target` (1 to the whole sum), the same in every CTA.
-    __device__ SampleFound find(bool mass, uint64_t target)
+    __device__ __forceinline__ int vectors() const { return n > 0 ? (n + skew + VEC - 1) / VEC : 0; }
+    // a thread's run of neighbouring vectors: an odd number, so that neighbouring threads read from different banks
+    __device__ __forceinline__ int run_length() const { return (vectors() + ST_THREADS - 1) / ST_THREADS | 1; }
+    __device__ __forceinline__ int run_begin(int thread) const { return min(thread * run_length(), vectors()); }
+    template <typename F>
+    __device__ __forceinline__ void run(F f) const { each(run_begin(threadIdx.x), 1, run_begin(threadIdx.x + 1), f); }
+    __device__ __forceinline__ uint64_t place(int i, float x) const { return ((uint64_t)st_key(x) << 32) | (uint32_t)(first + i); }
+    template <typename F>
+    __device__ __forceinline__ void all(F f) const { each(threadIdx.x, ST_THREADS, vectors(), f); }
+    __device__ __forceinline__ int coarse(float x) const { return st_coarse(x, max, scale); }
+
+    __device__ void clear(bool mass)
     {
+        uint32_t* w = s.word[0];
+        for (int i = threadIdx.x; i < (mass ? 3 : 1) * ST_BINS; i += ST_THREADS) w[i] = 0;
+        __syncthreads();
+    }
+    // adds a token to a histogram
+    __device__ __forceinline__ void put(bool mass, int bin, uint64_t weight)
+    {
+        if (!mass) {
+            atomicAdd(&s.word[0][bin], 1u);
+            return;
+        }
+        constexpr uint32_t mask = (1u << ST_LIMB) - 1;
+        const uint32_t lo = (uint32_t)weight & mask, mid = (uint32_t)(weight >> ST_LIMB) & mask, hi = (uint32_t)(weight >> (2 * ST_LIMB));
+        if (lo != 0) atomicAdd(&s.word[0][bin], lo);
+        if (mid != 0) atomicAdd(&s.word[1][bin], mid);
+        if (hi != 0) atomicAdd(&s.word[2][bin], hi);
+    }
+    // The bin in which the sums over the cluster's histograms reach goal(whole sum) (1 to the whole sum), the same in every CTA.
+    template <typename G>
+    __device__ SampleFound find(bool mass, G goal)
+    {
+        cl.sync();
         const int bins = ST_BINS / ranks, per = bins < ST_THREADS ? 1 : bins / ST_THREADS, at = rank * bins + threadIdx.x * per;
         const bool active = (int)threadIdx.x * per < bins;
-        uint64_t mine[4], sum = 0;
-        uint32_t counts[4];
+        uint64_t mine[4] = {0, 0, 0, 0}, sum = 0;
+        if (active)
+            for (int r = 0; r < ranks; r++) {
+                const SampleShared* o = cl.map_shared_rank(&s, r);
 #pragma unroll
-        for (int i = 0; i < 4; i++) {
-            mine[i] = 0;
-            counts[i] = 0;
-            if (active && i < per) {
-                for (int r = 0; r < ranks; r++) {
-                    const SampleShared* o = cl.map_shared_rank(&s, r);
-                    counts[i] += o->count[at + i];
-                    if (mass) mine[i] += o->lo[at + i] + ((uint64_t)o->hi[at + i] << 32);
-                }
-                if (!mass) mine[i] = counts[i];
-                sum += mine[i];
+                for (int i = 0; i < 4; i++)
+                    if (i < per) {
+                        mine[i] += o->word[0][at + i];
+                        if (mass) mine[i] += ((uint64_t)o->word[1][at + i] << ST_LIMB) + ((uint64_t)o->word[2][at + i] << (2 * ST_LIMB));
+                    }
             }
-        }
+#pragma unroll
+        for (int i = 0; i < 4; i++) sum += mine[i];
         uint64_t total;
         uint64_t before = st_scan(sum, s.scan, total);
         if ((int)threadIdx.x < ranks) cl.map_shared_rank(&s, threadIdx.x)->part[rank] = total;
         cl.sync();
-        for (int r = 0; r < rank; r++) before += s.part[r];
+        total = 0;
+        for (int r = 0; r < ranks; r++) {
+            if (r < rank) before += s.part[r];
+            total += s.part[r];
+        }
+        const uint64_t target = goal(total);
 #pragma unroll
         for (int i = 0; i < 4; i++) {
             if (active && i < per && before < target && target <= before + mine[i])
-                for (int r = 0; r < ranks; r++) cl.map_shared_rank(&s, r)->found = SampleFound{at + i, counts[i], before};
+                for (int r = 0; r < ranks; r++) cl.map_shared_rank(&s, r)->found = SampleFound{at + i, before};
             before += mine[i];
         }
         cl.sync();
         return s.found;
     }
-    // The key at which the tokens before it and `target` of its own (by count or by mass) make up `target`, among keys below `limit`; before: their sum.
-    __device__ uint32_t select(bool mass, uint64_t target, uint32_t limit, const SampleWeight& weight, float scale, uint64_t& before)
+    // Goes over the CTA's tokens a run a thread: where f(number, value) says so, a token is listed, in no order.  Then the cluster's lists are gathered into the first CTA's;
+    // their tokens' number, or -1 where they are too many.  The lists lie over the histograms.  (A barrier of the cluster before the others' lists change.)
+    template <typename F>
+    __device__ int gather(F f)
     {
-        const float max = weight.max;
-        auto coarse = [&](float x) {
-            const float d = x == max ? 0.0f : max - x;
-            return (int)fminf(d * scale, (float)(ST_BINS - 1));
-        };
-        histogram(mass, weight, [&](float x) { return st_key(x) < limit ? coarse(x) : -1; });
-        SampleFound f = find(mass, target);
-        before = f.before;
+        if (threadIdx.x == 0) s.mine = 0;
+        __syncthreads();
+        run([&](int i, float x) {
+            if (f(i, x)) {
+                const int at = atomicAdd(&s.mine, 1);
+                if (at < ST_LIST) s.list[at] = place(i, x);
+            }
+        });
+        __syncthreads();
+        if ((int)threadIdx.x < ranks) cl.map_shared_rank(&s, threadIdx.x)->listed[rank] = s.mine;
+        cl.sync();
+        int sum = 0;
+        bool fits = true;
+        for (int r = 0; r < ranks; r++) {
+            fits = fits && s.listed[r] <= ST_LIST;
+            sum += s.listed[r];
+        }
+        if (!fits || sum > ST_LIST) return -1;
+        if (rank == 0) {
+            for (int r = 1, at = s.listed[0]; r < ranks; at += s.listed[r++]) {
+                const uint64_t* from = cl.map_shared_rank(&s, r)->list;
+                for (int i = threadIdx.x; i < s.listed[r]; i += ST_THREADS) s.list[at + i] = from[i];
+            }
+            __syncthreads();
+        }
+        return sum;
+    }
+    __device__ void tell(uint64_t last)
+    {
+        for (int r = 0; r < ranks; r++) cl.map_shared_rank(&s, r)->cut = last;
+    }
+    // Among `count` listed tokens, in order: the one at which sums reach `rest`, told to the cluster.
+    __device__ void cut_list(bool mass, int count, uint64_t rest, const SampleWeight& weight)
+    {
+        const int tid = threadIdx.x;
+        if (tid < count) {
+            const uint64_t v = s.list[tid];
+            s.sorted[st_rank(s.list, count, v)] = v;
+        }
+        __syncthreads();
+        const uint64_t v = tid < count ? s.sorted[tid] : 0;
+        const uint64_t w = tid >= count ? 0 : mass ? weight(st_unkey((uint32_t)(v >> 32))) : 1;
+        uint64_t total;
+        const uint64_t before = st_scan(w, s.scan, total);
+        if (before < rest && rest <= before + w) tell(v);
+    }
+    // Finds the token at which, in order, sums of those up to `limit` reach goal(their whole sum), by number or by weight.  sum: the thread's run's weights from `least` on of
+    // the bins before the token's, for the draw.
+    template <typename G>
+    __device__ SampleCut select(bool mass, uint64_t limit, const SampleWeight& weight, uint64_t least, uint64_t& sum, G goal)
+    {
+        clear(mass);
+        all([&](int i, float x) {
+            if (limit == ~0ull || place(i, x) <= limit) put(mass, coarse(x), mass ? weight(x) : 0);
+        });
+        uint64_t target = 0;
+        SampleFound f = find(mass, [&](uint64_t whole) {
+            target = goal(whole);
+            return target;
+        });
         const int bin = f.bin;
-        if (!mass && bin == ST_BINS - 1) return ST_NO_CUT;      // weights of 2^-44 and less
+        if (!mass && bin == ST_BINS - 1) return SampleCut{limit, -1};      // weights of 2^-42 and less
+        uint64_t rest = target - f.before;
+        sum = 0;
+        int count = 0;
+        count = gather([&](int i, float x) {
+            const int b = coarse(x);
+            if (b > bin || (limit != ~0ull && place(i, x) > limit)) return false;
+            if (b < bin) {
+                const uint64_t w = weight(x);
+                if (w >= least) sum += w;
+            }
+            return b == bin;
+        });
+        if (count >= 0) {
+            if (rank == 0) cut_list(mass, count, rest, weight);
+            cl.sync();
+            return SampleCut{s.cut, bin};
+        }
+        // too many: the key by its bits, then the token by its number among the key's
         uint32_t prefix = 0;
 #pragma unroll 1
         for (int level = 0; level < 3; level++) {
             const int shift = level == 0 ? 21 : level == 1 ? 10 : 0, bits = level == 2 ? 10 : 11;
-            histogram(mass, weight, [&](float x) {
+            cl.sync();
+            clear(mass);
+            all([&](int i, float x) {
                 const uint32_t k = st_key(x);
-                if (k >= limit || coarse(x) != bin || (level > 0 && (k >> (shift + bits)) != prefix)) return -1;
-                return (int)((k >> shift) & ((1u << bits) - 1));
+                if (coarse(x) == bin && (level == 0 || (k >> (shift + bits)) == prefix) && place(i, x) <= limit)
+                    put(mass, (int)((k >> shift) & ((1u << bits) - 1)), mass ? weight(x) : 0);
             });
-            f = find(mass, target - before);
-            before += f.before;
+            f = find(mass, [&](uint64_t) { return rest; });
+            rest -= f.before;
             prefix = (prefix << bits) | (uint32_t)f.bin;
         }
-        return prefix;
+        if (mass) {
+            const uint64_t w = weight(st_unkey(prefix));
+            rest = (rest + w - 1) / w;
+        }
+        uint64_t ties = 0, total;
+        run([&](int, float x) { ties += st_key(x) == prefix ? 1 : 0; });
+        uint64_t before = st_scan(ties, s.scan, total);
+        if ((int)threadIdx.x < ranks) cl.map_shared_rank(&s, threadIdx.x)->part[rank] = total;
+        cl.sync();
+        for (int r = 0; r < rank; r++) before += s.part[r];
+        if (before < rest && rest <= before + ties)
+            run([&](int i, float x) {
+                if (st_key(x) == prefix && ++before == rest) tell(place(i, x));
+            });
+        cl.sync();
+        return SampleCut{s.cut, -1};
     }
 };
 
@@ -226,16 +482,24 @@ __global__ void __launch_bounds__(ST_THREADS) ns_sample_tokens_kernel(const Samp
     constexpr int VEC = 16 / sizeof(T);
     const int skew = (int)((reinterpret_cast<uintptr_t>(src) & 15) / sizeof(T));
     T* vals = reinterpret_cast<T*>(st_smem + sizeof(SampleShared)) + skew;
-    for (int i = tid; i < ST_TABLE; i += ST_THREADS) s.table[i] = exp2(-(double)i / ST_TABLE);
 
+    // asked for ahead of the row
+    const float temperature = p.temperature != nullptr ? p.temperature[row] : 1.0f;
+    int k = p.top_k != nullptr ? p.top_k[row] : 0;
+    const float top_p = p.top_p != nullptr ? p.top_p[row] : 1.0f, min_p = p.min_p != nullptr ? p.min_p[row] : 0.0f;
+    uint64_t power[ST_TABLE / ST_THREADS];
+#pragma unroll
+    for (int i = 0; i < ST_TABLE / ST_THREADS; i++) power[i] = st_powers.v[tid + i * ST_THREADS];
     float best = -INFINITY;
     int best_at = p.vocab;
     auto take = [&](T raw, int i) {
-        const float v = st_value(raw);
+        const T kept = st_clean(raw);
+        const float v = st_value(kept);
         if (v > best) { best = v; best_at = first + i; }
+        return kept;
     };
     const int head = min(n, skew == 0 ? 0 : VEC - skew), vecs = (n - head) / VEC, tail = head + vecs * VEC;
-    if (tid < head) { vals[tid] = src[tid]; take(src[tid], tid); }
+    if (tid < head) vals[tid] = take(src[tid], tid);
     {
         constexpr int U = 4;
         const uint4* from = reinterpret_cast<const uint4*>(src + head);
@@ -248,15 +512,20 @@ __global__ void __launch_bounds__(ST_THREADS) ns_sample_tokens_kernel(const Samp
 #pragma unroll
             for (int u = 0; u < U; u++)
                 if (at + u * ST_THREADS < vecs) {
-                    to[at + u * ST_THREADS] = v[u];
-                    const T* e = reinterpret_cast<const T*>(&v[u]);
+                    T* e = reinterpret_cast<T*>(&v[u]);
 #pragma unroll
-                    for (int i = 0; i < VEC; i++) take(e[i], head + (at + u * ST_THREADS) * VEC + i);
+                    for (int i = 0; i < VEC; i++) e[i] = take(e[i], head + (at + u * ST_THREADS) * VEC + i);
+                    to[at + u * ST_THREADS] = v[u];
                 }
         }
     }
-    if (tail + tid < n) { vals[tail + tid] = src[tail + tid]; take(src[tail + tid], tail + tid); }
+    if (tail + tid < n) vals[tail + tid] = take(src[tail + tid], tail + tid);
 
+#pragma unroll
+    for (int i = 0; i < ST_TABLE / ST_THREADS; i++) {
+        s.table.fixed[tid + i * ST_THREADS] = power[i];
+        s.table.value[tid + i * ST_THREADS] = (float)power[i];
+    }
     // ---- the first maximum
 #pragma unroll
     for (int o = 16; o > 0; o >>= 1) {
@@ -279,9 +548,6 @@ __global__ void __launch_bounds__(ST_THREADS) ns_sample_tokens_kernel(const Samp
     for (int r = 1; r < ranks; r++)
         if (st_better(s.max[r], s.max_at[r], max, max_at)) { max = s.max[r]; max_at = s.max_at[r]; }
 
-    const float temperature = p.temperature != nullptr ? p.temperature[row] : 1.0f;
-    int k = p.top_k != nullptr ? p.top_k[row] : 0;
-    const float top_p = p.top_p != nullptr ? p.top_p[row] : 1.0f, min_p = p.min_p != nullptr ? p.min_p[row] : 0.0f;
     if (k <= 0 || k > p.vocab) k = p.vocab;
     // greedily, or nothing to choose from: every CTA sees the same and leaves
     if (max == -INFINITY || !(temperature > 0.0f) || k == 1) {
@@ -291,108 +557,93 @@ __global__ void __launch_bounds__(ST_THREADS) ns_sample_tokens_kernel(const Samp
         }
         return;
     }
-    const SampleWeight weight{max, 184.6649652337873 / (double)temperature, s.table};       // 128 / ln 2
-    const float scale = fminf(64.0f / temperature, 1e30f);
-    SampleRow<T> me{p, s, vals, n, first, cl, rank, ranks};
-
-    // ---- cutoffs: kept are keys below `cut`, and the first `ties` tokens of key `cut`
-    uint32_t cut = ST_NO_CUT, ties = 0;
-    uint64_t tie_weight = 0;
-    auto mass_below = [&](uint32_t limit) {
-        uint64_t sum = 0, total;
-        for (int i = tid; i < n; i += ST_THREADS) {
-            const float x = st_value(vals[i]);
-            if (st_key(x) < limit) sum += weight(x);
-        }
-        st_scan(sum, s.scan2, total);
-        if (tid < ranks) cl.map_shared_rank(&s, tid)->mass[rank] = total;
-        cl.sync();
-        total = 0;
-        for (int r = 0; r < ranks; r++) total += s.mass[r];
-        return total;
-    };
-    auto key_weight = [&](uint32_t key) { return weight(__uint_as_float((key >> 31) ? key : ~key ^ 0x80000000u)); };
-    if (k < p.vocab) {
-        uint64_t before;
-        cut = me.select(false, (uint64_t)k, ST_NO_CUT, weight, scale, before);
-        if (cut != ST_NO_CUT) {
-            ties = (uint32_t)(k - before);
-            tie_weight = key_weight(cut);
-        }
-    }
-    if (top_p < 1.0f) {
-        const uint64_t above = mass_below(cut), all = above + ties * tie_weight;
-        uint64_t target = top_p > 0.0f ? (uint64_t)ceil((double)top_p * (double)all) : 1;
-        if (target == 0) target = 1;
-        uint64_t before = above;
-        if (target <= above) {
-            cut = me.select(true, target, cut, weight, scale, before);
-            tie_weight = key_weight(cut);
-            ties = 0xFFFFFFFFu;
-        }
-        // the fewest tokens of the cutoff's weight that reach the target
-        if (tie_weight != 0) ties = (uint32_t)min((uint64_t)ties, (target - before + tie_weight - 1) / tie_weight);
-    }
+    const SampleWeight weight(max, temperature, &s.table);
+    SampleRow<T> me{s, vals, n, first, skew, cl, rank, ranks, max, fminf(64.0f / temperature, 1e30f)};
     uint64_t least = 0;
     if (min_p > 0.0f) least = (uint64_t)ceil((double)fminf(min_p, 1.0f) * (double)(1ull << ST_FIX));
-    if (tie_weight < least) ties = 0;
 
-    // ---- the draw: runs of neighbouring tokens, one a thread, in the vocabulary's order
-    const int seg = (p.each + ST_THREADS - 1) / ST_THREADS | 1, j0 = min(tid * seg, n), j1 = min(j0 + seg, n);
-    uint64_t sum = 0, tie_count = 0;
-    for (int j = j0; j < j1; j++) {
-        const float x = st_value(vals[j]);
-        const uint32_t key = st_key(x);
-        if (key < cut) {
-            const uint64_t w = weight(x);
-            if (w >= least) sum += w;
-        } else if (key == cut) {
-            tie_count++;
+    // ---- few candidates
+    if (k <= ST_SORT_K && k < p.vocab) {
+        // from a sample: so much of it that k tokens hardly ever fail to be among those it stands for
+        int every = 1;
+        uint64_t need = k;
+        if (p.vocab > 1024 * ST_SAMPLE) {
+            every = ST_SAMPLE;
+            const float share = (float)k / ST_SAMPLE;
+            need = (uint64_t)(1.25f * share + 3.0f * sqrtf(share) + 4.0f);
         }
+        me.clear(false);
+        for (int i = (every - first % every) % every + tid * every; i < n; i += ST_THREADS * every) me.put(false, me.coarse(st_value(vals[i])), 0);
+        const int bin = me.find(false, [&](uint64_t sample) { return need < sample ? need : sample; }).bin;
+        int count = 0;
+        count = me.gather([&](int, float x) { return me.coarse(x) <= bin; });
+        if (count >= k) {
+            cl.sync();                     // the first CTA has the others' lists
+            if (rank != 0) return;
+            const SampleCuts cuts{k, top_p, p.u[row], least};
+            st_draw(s, count, cuts, weight, row, p);
+            return;
+        }
+        cl.sync();
     }
-    uint64_t all_sum, all_ties;
-    __syncthreads();
-    uint64_t before = st_scan(sum, s.scan, all_sum), ties_before = st_scan(tie_count, s.scan2, all_ties);
-    if (tid < ranks) {
-        SampleShared* o = cl.map_shared_rank(&s, tid);
-        o->part[rank] = all_sum;
-        o->ties[rank] = all_ties;
+
+    // ---- cutoffs
+    SampleCut cut{~0ull, -1};
+    uint64_t sum = 0;
+    if (k < p.vocab) cut = me.select(false, cut.last, weight, least, sum, [&](uint64_t) { return (uint64_t)k; });
+    if (top_p < 1.0f) {
+        cl.sync();
+        cut = me.select(true, cut.last, weight, least, sum, [&](uint64_t whole) { return st_goal(top_p, whole); });
     }
+
+    // ---- the draw: the weights of each thread's run
+    auto kept = [&](int i, float x) {
+        const uint64_t w = cut.last == ~0ull || me.place(i, x) <= cut.last ? weight(x) : 0;
+        return w >= least ? w : 0;
+    };
+    if (cut.bin < 0) {
+        sum = 0;
+        me.run([&](int i, float x) { sum += kept(i, x); });
+    } else {
+        // all but the cutoff's bin are in the sums: its tokens are this CTA's part of the lists
+        s.extra[tid] = 0;
+        __syncthreads();
+        if (tid < s.mine) {
+            const uint64_t v = s.list[tid];
+            if (v <= cut.last) {
+                const uint64_t w = weight(st_unkey((uint32_t)(v >> 32)));
+                const int thread = ((int)(uint32_t)v - first + skew) / me.VEC / me.run_length();
+                if (w >= least) atomicAdd(reinterpret_cast<unsigned long long*>(&s.extra[thread]), (unsigned long long)w);
+            }
+        }
+        __syncthreads();
+        sum += s.extra[tid];
+    }
+    uint64_t total;
+    uint64_t before = st_scan(sum, s.scan, total);
+    if (tid < ranks) cl.map_shared_rank(&s, tid)->draw[rank] = total;
     cl.sync();
-    all_sum = 0;
-    all_ties = 0;
+    total = 0;
     for (int r = 0; r < ranks; r++) {
-        if (r < rank) { before += s.part[r]; ties_before += s.ties[r]; }
-        all_sum += s.part[r];
-        all_ties += s.ties[r];
+        if (r < rank) before += s.draw[r];
+        total += s.draw[r];
     }
-    const uint64_t kept_ties = ties;
-    const uint64_t total = all_sum + min(all_ties, kept_ties) * tie_weight;
-    const float u = p.u[row];
-    // a running sum exceeds u * total where it exceeds that number's floor
-    uint64_t target = u < 1.0f ? (u > 0.0f ? (uint64_t)((double)u * (double)total) : 0) : total - 1;
-    if (target >= total) target = total - 1;
-    uint64_t run = before + min(ties_before, kept_ties) * tie_weight;
-    const uint64_t after = run + sum + (min(ties_before + tie_count, kept_ties) - min(ties_before, kept_ties)) * tie_weight;
-    if (run <= target && target < after) {
-        uint64_t tie = ties_before;
-        for (int j = j0; j < j1; j++) {
-            const float x = st_value(vals[j]);
-            const uint32_t key = st_key(x);
-            uint64_t w = 0;
-            if (key < cut) {
-                w = weight(x);
-                if (w < least) w = 0;
-            } else if (key == cut) {
-                if (tie < kept_ties) w = tie_weight;
-                tie++;
-            }
-            run += w;
-            if (run > target) {
-                p.ids[row] = first + j;
-                if (p.probs != nullptr) p.probs[row] = (float)((double)w / (double)total);
-                break;
-            }
+    const uint64_t aim = st_aim(p.u[row], total);
+    const bool mine = before <= aim && aim < before + sum;
+    // One run of the cluster's holds the token: its CTA goes over it a token a thread.
+    if (mine) {
+        s.run_first = me.run_begin(tid);
+        s.run_end = me.run_begin(tid + 1);
+        s.run_before = before;
+    }
+    if (__syncthreads_or(mine)) {
+        const int i = s.run_first * me.VEC - skew + tid;
+        uint64_t w = 0, unused;
+        if (i >= 0 && i < n && i < s.run_end * me.VEC - skew) w = kept(i, st_value(vals[i]));
+        const uint64_t at = s.run_before + st_scan(w, s.scan2, unused);
+        if (at <= aim && aim < at + w) {
+            p.ids[row] = first + i;
+            if (p.probs != nullptr) p.probs[row] = (float)((double)w / (double)total);
         }
     }
     cl.sync();      // a CTA's shared memory stays until the others have written to it
@@ -431,10 +682,11 @@ extern "C" int ns_sample_tokens(ns_device_t h, uint64_t logits, int dtype, int64
     p.u = reinterpret_cast<const float*>(u);
     p.ids = reinterpret_cast<int32_t*>(ids);
     p.probs = reinterpret_cast<float*>(probs);
-    // CTAs a row: until the SMs are full or a thread has few tokens left, and as many as its shared memory takes
+    // CTAs a row: as many as leave room for two of them an SM (one has too few warps for the latency of its passes: 256 rows of 131 001 bf16 NNN us with two a row,
+    // NNN with four), and until the SMs are full or a thread has few tokens left.
     int ranks = 1;
     auto each = [&](int r) { return ((vocab + r - 1) / r + 7) / 8 * 8; };
-    while (ranks < ST_MAX_CLUSTER && (each(ranks) > most_each || ((int64_t)rows * ranks < d->sm_count && each(ranks) > 8 * ST_THREADS))) ranks *= 2;
+    while (ranks < ST_MAX_CLUSTER && (2 * st_bytes(each(ranks), size) > (size_t)most || ((int64_t)rows * ranks < d->sm_count && each(ranks) > 8 * ST_THREADS))) ranks *= 2;
     p.each = each(ranks);
     const size_t smem = st_bytes(p.each, size);
     auto kernel = dtype == NS_F32 ? ns_sample_tokens_kernel<float> : ns_sample_tokens_kernel<uint16_t>;

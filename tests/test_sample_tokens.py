@@ -158,8 +158,8 @@ def test_refusals():
 
     call("device handle is null")
     call("device handle is null", rows=0)
-    call("device handle is null", vocab=408000)
-    call("device handle is null", vocab=816000, dtype=N.NS_BF16)
+    call("device handle is null", vocab=380000)
+    call("device handle is null", vocab=760000, dtype=N.NS_BF16)
     for name in ("x", "u", "ids"):
         call("null argument", **{name: 0})
     call("dtype", dtype=N.NS_I8)
