@@ -11,6 +11,7 @@
 #include <type_traits>
 
 #include "ns_cache.cuh"
+#include "ns_mma.cuh"
 #include "ns_seq.cuh"
 
 namespace {
@@ -299,7 +300,8 @@ struct AppendArgs {
     uint16_t* k_pool;
     uint16_t* v_pool;
     int lane_tasks;                        // lanes a head, at most 32
-    int parts;                             // warps a row, each a share of its heads and vectors
+    int parts, heads_each;                 // warps a row, and heads of each
+    int stage_at;                          // bytes: where the warps' source heads lie in shared memory, behind their angles
     RotDiv rest, value;                    // vectors of a head that are not turned, and of a value head
     int* status;
 };
@@ -334,16 +336,18 @@ __device__ __forceinline__ void rot_store(uint16_t* dst, const RotVec<float, VEC
     rot_store<VEC>(dst, o);
 }
 
-// A warp a row, or several where there are few rows; no barrier joins them.  What a token's place and angles come from is a chain of three loads (position, page, data), so what
-// counts is that many warps are at different links of it.
+// A warp a row, or several, each with a range of its heads (queries, keys, values); no barrier joins them.  What a token's place and angles come from is a chain of
+// three loads (position, page, data), so what counts is that many bytes are on their way: a bf16 source's heads all at once, through shared memory.  (Through registers,
+// four vectors a lane at a time, 13 x 777 tokens of 48 heads x 128 took 42 us, with two warps a row 34; so they take 26, 4.7 TB/s.)
 template <bool HALVES, int VEC, int SLABS>
 __global__ void __launch_bounds__(ROT_THREADS, SLABS == NS_TOGETHER ? 1 : SLABS == ROT_BF16 ? 4 : 3) ns_kv_append_rotary_kernel(const AppendArgs p)
 {
     using N = RotTasks<HALVES, VEC>;
     using H = RotHeld<VEC, SLABS>;
+    constexpr bool STAGED = SLABS == ROT_BF16 && VEC == 8;
     constexpr int U = SLABS == NS_TOGETHER ? 1 : SLABS == ROT_BF16 && !N::TWO ? 4 : 2;      // heads a lane has on their way
     constexpr int K = SLABS == NS_TOGETHER ? 1 : SLABS == ROT_BF16 ? 4 : 2;                 // vectors to copy
-    extern __shared__ float2 rot_table[];
+    extern __shared__ __align__(16) uint8_t rot_smem[];
     ns_pdl_wait();
     ns_pdl_trigger();
     const N n(p.dim, p.rot);
@@ -353,47 +357,68 @@ __global__ void __launch_bounds__(ROT_THREADS, SLABS == NS_TOGETHER ? 1 : SLABS 
     const int b = r / p.steps, i = r - b * p.steps;
     const int first_pos = p.pos[b], offset = p.offset != nullptr ? p.offset[0] : 0;
     if (p.lens != nullptr && i >= p.lens[b]) return;
+    // this warp's heads: turned ones below `all_heads`, values behind
+    const int all_heads = p.heads + p.kv_heads, head0 = part * p.heads_each, head1 = min(head0 + p.heads_each, all_heads + p.kv_heads);
+    const int64_t src0 = (int64_t)r * p.src.ld, head_step = (int64_t)p.dim << p.page_shift;
+    auto column = [&](int head) {
+        return head < p.heads ? p.q_col + head * p.dim : head < all_heads ? p.k_col + (head - p.heads) * p.dim : p.v_col + (head - all_heads) * p.dim;
+    };
+    float2* table = reinterpret_cast<float2*>(rot_smem) + warp * n.table();
+    const uint16_t* staged = reinterpret_cast<const uint16_t*>(rot_smem + p.stage_at) + warp * p.heads_each * p.dim;
+    if constexpr (STAGED) {
+        const int per = p.dim / 8, total = (head1 - head0) * per;
+        const uint16_t* src = reinterpret_cast<const uint16_t*>(p.src.ptr) + src0;
+        for (int e = lane; e < total; e += 32) {
+            const int head = p.value.of(e), c = (e - head * per) * 8;
+            ns_cp_async16(ns_smem_u32(staged + head * p.dim + c), src + column(head0 + head) + c);
+        }
+        ns_cp_commit();
+    }
     // positions in 64 bits: nothing wraps around
     const int64_t at = (int64_t)first_pos + i;
     int page = -1;
     if (at >= 0 && (at >> p.page_shift) < p.max_pages) page = p.page_table[(int64_t)b * p.max_pages + (at >> p.page_shift)];
-    const int64_t src0 = (int64_t)r * p.src.ld, head_step = (int64_t)p.dim << p.page_shift;
+    auto read = [&](int head, int c, H& v) {
+        if constexpr (STAGED) v = *reinterpret_cast<const H*>(staged + (head - head0) * p.dim + c);
+        else rot_source<VEC, SLABS>(p.src, src0 + column(head) + c, v);
+    };
 
     // ---- turned heads: lanes of a head, heads side by side
-    const int across = 32 / p.lane_tasks, t0 = lane % p.lane_tasks, sub = lane / p.lane_tasks, step = across * p.parts;
-    const int all_heads = p.heads + p.kv_heads;
-    auto source = [&](int head) { return src0 + (head < p.heads ? p.q_col + head * p.dim : p.k_col + (head - p.heads) * p.dim); };
+    const int across = 32 / p.lane_tasks, t0 = lane % p.lane_tasks, sub = lane / p.lane_tasks;
     H x[U], y[U];
     auto load = [&](int t, int h) {
 #pragma unroll
         for (int u = 0; u < U; u++)
-            if (h + u * step < all_heads) {
-                const int64_t src = source(h + u * step) + n.first(t);
-                rot_source<VEC, SLABS>(p.src, src, x[u]);
-                if (N::TWO) rot_source<VEC, SLABS>(p.src, src + n.second(), y[u]);
+            if (h + u * across < min(head1, all_heads)) {
+                read(h + u * across, n.first(t), x[u]);
+                if (N::TWO) read(h + u * across, n.first(t) + n.second(), y[u]);
             }
     };
     const bool mine = sub < across;
-    const int h0 = part * across + sub;
-    if (mine) load(t0, h0);
-    float2* table = rot_table + warp * n.table();
-    for (int e = lane; e < half; e += 32) table[n.slot(e)] = rot_cos_sin((double)(at + offset), p.freq[e], p.amplitude);
+    const int h0 = head0 + sub;
+    if (!STAGED && mine) load(t0, h0);
+    if (head0 < all_heads)
+        for (int e = lane; e < half; e += 32) table[n.slot(e)] = rot_cos_sin((double)(at + offset), p.freq[e], p.amplitude);
+    if constexpr (STAGED) ns_cp_wait<0>();
     __syncwarp();
     const bool stored = page >= 0 && page < p.num_pages;
     if (!stored && lane == 0) *reinterpret_cast<volatile int*>(p.status) = 500;
     const int64_t slab = (((int64_t)page * p.kv_heads << p.page_shift) + (at & ((1 << p.page_shift) - 1))) * p.dim;      // head 0's row in the page
-    auto target = [&](int head) { return head < p.heads ? p.q + (int64_t)r * p.q_ld + (int64_t)head * p.dim : p.k_pool + slab + (int64_t)(head - p.heads) * head_step; };
-    const int heads = stored ? all_heads : p.heads;
+    auto target = [&](int head) {
+        return head < p.heads ? p.q + (int64_t)r * p.q_ld + (int64_t)head * p.dim
+                              : (head < all_heads ? p.k_pool + (int64_t)(head - p.heads) * head_step : p.v_pool + (int64_t)(head - all_heads) * head_step) + slab;
+    };
+    const int end = min(head1, stored ? all_heads : p.heads);
     if (mine) {
         for (int t = t0; t < n.turned; t += p.lane_tasks) {
             float2 w[N::PAIRS];
             n.angles(table, t, w);
-            if (t != t0) load(t, h0);
-            for (int h = h0; h < heads; h += U * step) {
+            if (STAGED || t != t0) load(t, h0);
+            for (int h = h0; h < end; h += U * across) {
 #pragma unroll
                 for (int u = 0; u < U; u++)
-                    if (h + u * step < heads) {
-                        uint16_t* dst = target(h + u * step) + n.first(t);
+                    if (h + u * across < end) {
+                        uint16_t* dst = target(h + u * across) + n.first(t);
                         float fa[VEC], fb[VEC];
                         rot_unpack(x[u], fa);
                         if (N::TWO) rot_unpack(y[u], fb);
@@ -406,34 +431,39 @@ __global__ void __launch_bounds__(ROT_THREADS, SLABS == NS_TOGETHER ? 1 : SLABS 
                             rot_store<VEC>(dst + n.second(), o);
                         }
                     }
-                load(t, h + U * step);
+                load(t, h + U * across);
             }
         }
     }
     // ---- what is not turned of those heads, and the values
     H v[K];
     auto copy = [&](int count, auto where) {
-        for (int e = part * 32 + lane; e < count; e += K * 32 * p.parts) {
+        for (int e = lane; e < count; e += K * 32) {
             uint16_t* to[K];
 #pragma unroll
             for (int u = 0; u < K; u++)
-                if (e + u * 32 * p.parts < count) rot_source<VEC, SLABS>(p.src, where(e + u * 32 * p.parts, to[u]), v[u]);
+                if (e + u * 32 < count) {
+                    int c;
+                    const int head = where(e + u * 32, c);
+                    read(head, c, v[u]);
+                    to[u] = target(head) + c;
+                }
 #pragma unroll
             for (int u = 0; u < K; u++)
-                if (e + u * 32 * p.parts < count) rot_store<VEC>(to[u], v[u]);
+                if (e + u * 32 < count) rot_store<VEC>(to[u], v[u]);
         }
     };
     const int rest = (p.dim - n.rest) / VEC;
-    copy(heads * rest, [&](int e, uint16_t*& to) {
-        const int head = p.rest.of(e), c = n.rest + (e - head * rest) * VEC;
-        to = target(head) + c;
-        return source(head) + c;
+    copy(max(end - head0, 0) * rest, [&](int e, int& c) {
+        const int head = p.rest.of(e);
+        c = n.rest + (e - head * rest) * VEC;
+        return head0 + head;
     });
-    const int per = p.dim / VEC;
-    copy(stored ? p.kv_heads * per : 0, [&](int e, uint16_t*& to) {
-        const int head = p.value.of(e), c = (e - head * per) * VEC;
-        to = p.v_pool + slab + head * head_step + c;
-        return src0 + p.v_col + head * p.dim + c;
+    const int per = p.dim / VEC, value0 = max(head0, all_heads);
+    copy(stored ? max(head1 - value0, 0) * per : 0, [&](int e, int& c) {
+        const int head = p.value.of(e);
+        c = (e - head * per) * VEC;
+        return value0 + head;
     });
 }
 
@@ -557,16 +587,25 @@ extern "C" int ns_kv_append_rotary(ns_device_t h, ns_kv_cache_t cache, uint64_t 
         constexpr int VEC = decltype(vc)::value;
         const RotTasks<HALVES, VEC> n(dim, rot_dims);
         p.lane_tasks = n.turned < 32 ? n.turned : 32;
-        // few rows: until there are eight warps an SM, or each has one turn
-        const int turns = (heads + c.heads + 32 / p.lane_tasks - 1) / (32 / p.lane_tasks);
-        p.parts = 1;
-        while ((int64_t)rows * p.parts < 8 * d->sm_count && p.parts < turns) p.parts *= 2;
+        // Warps a row: two where rows are many (one: 41 us for 13 x 777, four: 37), more for few rows, until there are eight warps an SM or each has one turn, and
+        // for rows that the staging memory of a warp does not hold.
+        const int row_heads = heads + 2 * c.heads, across = 32 / p.lane_tasks;
+        const bool staged = src_dtype == NS_BF16 && VEC == 8;
+        constexpr int stage_bytes = 6144;
+        p.parts = 2;
+        while (p.parts < row_heads && ((int64_t)rows * p.parts < 8 * d->sm_count ? row_heads > p.parts * across
+                                                                                 : staged && (row_heads + p.parts - 1) / p.parts * dim * 2 > stage_bytes))
+            p.parts *= 2;
+        p.heads_each = (row_heads + p.parts - 1) / p.parts;
+        p.parts = (row_heads + p.heads_each - 1) / p.heads_each;
         p.rest = RotDiv((dim - n.rest) / VEC);
         p.value = RotDiv(dim / VEC);
         const int64_t items = (int64_t)rows * p.parts;
-        const size_t smem = (size_t)(ROT_THREADS / 32) * n.table() * sizeof(float2);
+        p.stage_at = (ROT_THREADS / 32 * n.table() * (int)sizeof(float2) + 15) / 16 * 16;
+        const size_t smem = p.stage_at + (staged ? (size_t)(ROT_THREADS / 32) * p.heads_each * dim * 2 : 0);
         const dim3 grid((unsigned)((items + ROT_THREADS / 32 - 1) / (ROT_THREADS / 32)));
         auto launch = [&](auto kernel) {
+            NS_CUDA(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, 160 * 1024));
             NS_CUDA(ns_launch_plain(kernel, grid, dim3(ROT_THREADS), smem, d->stream, p));
             return (int)NS_OK;
         };
