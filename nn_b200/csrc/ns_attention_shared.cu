@@ -254,7 +254,13 @@ __global__ void __launch_bounds__(SH_THREADS, 3) ns_attention_shared_walk_kernel
     }
 }
 
-// The parts of every row fold, in order: a warp a row.
+template <int N>
+struct alignas(4 * N) ShColumns {
+    float v[N];
+};
+
+// The parts of every row fold, in order: a warp a row.  A lane weighs a part, 32 of them at a time; then every lane adds up its columns, whose loads do not wait for the
+// weights.
 template <int DH>
 __global__ void __launch_bounds__(256) ns_attention_shared_fold_kernel(const SharedParams p)
 {
@@ -269,22 +275,42 @@ __global__ void __launch_bounds__(256) ns_attention_shared_fold_kernel(const Sha
     const int token = r / p.group, i = token % p.steps;
     if (p.lens != nullptr && i >= p.lens[token / p.steps]) return;
     const int64_t step = (int64_t)p.kv_heads * rows_all;
-    float M = -INFINITY;
-    for (int k = lane; k < parts; k += 32) M = fmaxf(M, p.part_ml[idx + k * step].x);
-#pragma unroll
-    for (int o = 16; o > 0; o >>= 1) M = fmaxf(M, __shfl_xor_sync(0xffffffffu, M, o));
-    float L = 0.0f, O[N];
+    const float* src = p.part_o + idx * DH + lane * N;
+    float M = -INFINITY, L = 0.0f, O[N];
 #pragma unroll
     for (int n = 0; n < N; n++) O[n] = 0.0f;
-#pragma unroll 4
-    for (int k = 0; k < parts; k++) {
-        const float2 ml = p.part_ml[idx + k * step];
-        if (ml.x == -INFINITY && ml.y == 0.0f) continue;       // (its values were not written)
-        const float f = ml.x == -INFINITY ? 1.0f : ns_exp2(ml.x - M);
-        L = fmaf(ml.y, f, L);
-        const float* src = p.part_o + (idx + k * step) * DH + lane * N;
+    for (int k0 = 0; k0 < parts; k0 += 32) {
+        const int count = min(32, parts - k0);
+        const float2 ml = lane < count ? p.part_ml[idx + (k0 + lane) * step] : make_float2(-INFINITY, 0.0f);
+        float m = ml.x;
 #pragma unroll
-        for (int n = 0; n < N; n++) O[n] = fmaf(src[n], f, O[n]);
+        for (int o = 16; o > 0; o >>= 1) m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, o));
+        // (fmaxf leaves a maximum of NaN out; the part's sum is NaN then, and so is the row)
+        const float up = fmaxf(M, m), old = M == up ? 1.0f : ns_exp2(M - up);
+        const bool none = ml.x == -INFINITY && ml.y == 0.0f;         // (its values were not written)
+        const float f = none ? 0.0f : ml.x == -INFINITY ? 1.0f : ns_exp2(ml.x - up);
+        float l = none ? 0.0f : ml.y * f;
+#pragma unroll
+        for (int o = 16; o > 0; o >>= 1) l += __shfl_xor_sync(0xffffffffu, l, o);
+        L = fmaf(L, old, l);
+#pragma unroll
+        for (int n = 0; n < N; n++) O[n] *= old;
+        M = up;
+        const uint32_t there = __ballot_sync(0xffffffffu, !none);
+        for (int k = 0; k < count; k += 8) {
+            ShColumns<N> v[8];
+#pragma unroll
+            for (int u = 0; u < 8; u++)
+                if ((there >> (k + u)) & 1u) v[u] = *reinterpret_cast<const ShColumns<N>*>(src + (k0 + k + u) * step * DH);
+#pragma unroll
+            for (int u = 0; u < 8; u++) {
+                const float w = __shfl_sync(0xffffffffu, f, (k + u) & 31);
+                if ((there >> (k + u)) & 1u) {
+#pragma unroll
+                    for (int n = 0; n < N; n++) O[n] = fmaf(v[u].v[n], w, O[n]);
+                }
+            }
+        }
     }
     const float inv = L == 0.0f ? 0.0f : 1.0f / L;
     uint16_t* dst = p.o + (int64_t)token * p.o_stride + (int64_t)(kvh * p.group + r % p.group) * DH + lane * N;

@@ -560,11 +560,12 @@ __global__ void __launch_bounds__(ST_THREADS, 1) ns_attention_shared_tile_kernel
     }
 }
 
-// CTAs, by the longest prefix: the SMs, or a unit each.
+// CTAs, by the longest prefix.
 int tile_ctas(const NsDevice* d, const TileParams& p)
 {
     const int64_t blocks = (((int64_t)p.s.prefix_pages << p.s.page_shift) + ST_KB - 1) / ST_KB, units = blocks * p.tiles * p.s.kv_heads;
-    return (int)(units < d->sm_count ? units : d->sm_count);
+    // (two units each where there are fewer than that: a part costs its results' way through memory)
+    return (int)((units + 1) / 2 < d->sm_count ? (units + 1) / 2 : d->sm_count);
 }
 
 void tile_plan(const NsDevice* d, const SharedParams& s, TileParams& p)
