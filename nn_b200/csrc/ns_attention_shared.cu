@@ -19,7 +19,6 @@ namespace {
 constexpr int SH_WARPS = 4;
 constexpr int SH_THREADS = 32 * SH_WARPS;
 constexpr int SH_KEYS = 16;                // keys a warp takes at a time
-constexpr int SH_ROWS = 16;                // query rows of a CTA
 constexpr int SH_STAGES = 2;
 
 // 16 bytes to shared memory, zeros where there is nothing
@@ -29,21 +28,31 @@ __device__ __forceinline__ void sh_copy16(uint32_t dst, const void* src, bool th
     asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(dst), "l"(src), "r"(n) : "memory");
 }
 
-// A CTA: 16 rows of one key/value head against a range of keys.  Each warp walks 16 keys at a time on its own, through a ring of its own in shared memory, with
-// its own running maximum and sum; the four warps' results fold at the end.  P.V takes the weights as two bf16 halves: the rounding of
-// the output is then the only one that shows.
-template <int DH>
+// (8 x 8 of 16-bit values, a register a lane: rows become columns)
+__device__ __forceinline__ uint32_t sh_transpose(uint32_t v)
+{
+    uint32_t r;
+    asm volatile("movmatrix.sync.aligned.m8n8.trans.b16 %0, %1;" : "=r"(r) : "r"(v));
+    return r;
+}
+
+// A CTA: 8 NT rows of one key/value head against a range of keys.  Each warp walks 16 keys at a time on its own, through a ring of its own in shared memory, with
+// its own running maximum and sum; the four warps' results fold at the end.  The keys are the M of the products, S' = K Q' and O' = V' P', so that a group of up
+// to 8 query heads fills the N of 8: with the queries as M, 16 rows of which 4 are used, the MMAs took twice as long and bounded the kernel (34 GB/s an SM).
+// P.V takes the weights as two bf16 halves: the rounding of the output is then the only one that shows.
+template <int DH, int NT>
 __global__ void __launch_bounds__(SH_THREADS, 3) ns_attention_shared_walk_kernel(const SharedParams p)
 {
+    constexpr int ROWS = 8 * NT;
     constexpr int LD = DH + 8;                         // elements a row in shared memory: ldmatrix without conflicts
     constexpr int TILE = SH_KEYS * LD * 2;             // bytes
     constexpr int CHUNKS = DH / 8;                     // 16-byte pieces of a row
     constexpr int PASS = 32 / CHUNKS;                  // rows a warp copies at once
     extern __shared__ __align__(16) uint8_t sh_smem[];
     __shared__ uint32_t masks[SH_WARPS][SH_STAGES];
-    __shared__ float2 fold[SH_WARPS][SH_ROWS];
-    ns_pdl_wait();
-    ns_pdl_trigger();
+    __shared__ float2 fold[SH_WARPS][ROWS];
+    // (beside the tensor-core kernel, which needs the whole of the SMs it has: what came before that has completed, and nothing here needs its results)
+    if (p.beside == nullptr) ns_pdl_wait();
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
 
     // ---- which rows and which keys
@@ -57,7 +66,7 @@ __global__ void __launch_bounds__(SH_THREADS, 3) ns_attention_shared_walk_kernel
     const int kvh = item % p.kv_heads, b = item / p.kv_heads;       // b: 0 for the prefix
     const int rows_all = p.batch * p.steps * p.group;
     const int seq_rows = p.steps * p.group;
-    const int row0 = (prefix ? 0 : b * seq_rows) + tile * SH_ROWS;
+    const int row0 = (prefix ? 0 : b * seq_rows) + tile * ROWS;
     const int row_end = prefix ? rows_all : (b + 1) * seq_rows;
     const int part = prefix ? split : p.prefix_parts + split;
     const int32_t* table = prefix ? p.prefix_table : p.page_table + (int64_t)b * p.max_pages;
@@ -70,165 +79,200 @@ __global__ void __launch_bounds__(SH_THREADS, 3) ns_attention_shared_walk_kernel
         const int i = (r - b * seq_rows) / p.group;
         return i < own_len ? sh_clamp(own_pos + i, table_pages, p.page_shift) : 0;
     };
-    int n_keys;
+    // lane (g, t) = (lane / 4, lane % 4): keys g and g + 8 of a tile, rows 2 t and 2 t + 1 of each 8
+    const int fg = lane >> 2, ft = lane & 3;
+    int limit[2 * NT], n_keys;
     if (prefix) {
         n_keys = sh_clamp(p.prefix_len[0], table_pages, p.page_shift);
+#pragma unroll
+        for (int e = 0; e < 2 * NT; e++) limit[e] = n_keys;
     } else {
         n_keys = 0;
-        for (int r = row0; r < min(row0 + SH_ROWS, row_end); r += p.group) n_keys = max(n_keys, seen(r));
-        n_keys = max(n_keys, seen(min(row0 + SH_ROWS, row_end) - 1));
+#pragma unroll
+        for (int e = 0; e < 2 * NT; e++) {
+            limit[e] = seen(row0 + (e >> 1) * 8 + ft * 2 + (e & 1));
+            n_keys = max(n_keys, limit[e]);
+        }
+        n_keys = max(n_keys, __shfl_xor_sync(0xffffffffu, n_keys, 1));
+        n_keys = max(n_keys, __shfl_xor_sync(0xffffffffu, n_keys, 2));
     }
     const int tiles_all = (n_keys + SH_KEYS - 1) / SH_KEYS, per = (tiles_all + splits - 1) / splits;
     const int t0 = min(split * per, tiles_all), t1 = min(t0 + per, tiles_all);
-
-    // ---- queries: A fragments of 16 rows
-    const int fr = lane >> 2, fc = (lane & 3) * 2;
-    uint32_t qf[DH / 16][4];
-    {
-        const uint16_t* qr[2];
-#pragma unroll
-        for (int h = 0; h < 2; h++) {
-            const int r = row0 + fr + 8 * h;
-            qr[h] = r < row_end ? p.q + (int64_t)(r / p.group) * p.q_stride + (int64_t)(kvh * p.group + r % p.group) * DH : nullptr;
-        }
-#pragma unroll
-        for (int kk = 0; kk < DH / 16; kk++)
-#pragma unroll
-            for (int e = 0; e < 4; e++)
-                qf[kk][e] = qr[e & 1] != nullptr ? *reinterpret_cast<const uint32_t*>(qr[e & 1] + kk * 16 + fc + (e >> 1) * 8) : 0u;
-    }
-    int limit[2] = {n_keys, n_keys};
-    if (!prefix) {
-        limit[0] = seen(row0 + fr);
-        limit[1] = seen(row0 + fr + 8);
-    }
 
     // ---- keys and values
     const uint32_t ring = ns_smem_u32(sh_smem) + warp * SH_STAGES * 2 * TILE;
     const int64_t head_off = (int64_t)kvh << p.page_shift;
     const int page_mask = (1 << p.page_shift) - 1;
-    auto load = [&](int t, int stage) {
+    // the page of key lane % 16 of tile t, -1 behind the last; and its cached row as an element of the pools, or -1
+    auto page_of = [&](int t) {
+        const int j = t * SH_KEYS + (lane & 15);
+        return t < t1 && j < n_keys ? table[j >> p.page_shift] : -1;
+    };
+    auto locate = [&](int t, int page) {
+        const int j = t * SH_KEYS + (lane & 15);
+        if (t >= t1 || j >= n_keys) return (int64_t)-1;
+        if (page < 0 || page >= p.num_pages) {
+            *reinterpret_cast<volatile int*>(p.status) = SH_BAD_PAGE;
+            return (int64_t)-1;
+        }
+        return ((((int64_t)page * p.kv_heads) << p.page_shift) + head_off + (j & page_mask)) * DH;
+    };
+    auto load = [&](int t, uint32_t dst, const uint16_t* pool, int64_t at) {
         if (t < t1) {
-            // the cached row of key t * 16 + lane % 16, or -1
-            const int j = t * SH_KEYS + (lane & 15);
-            int64_t at = -1;
-            if (j < n_keys) {
-                const int page = table[j >> p.page_shift];
-                if (page >= 0 && page < p.num_pages) at = ((((int64_t)page * p.kv_heads) << p.page_shift) + head_off + (j & page_mask)) * DH;
-                else *reinterpret_cast<volatile int*>(p.status) = SH_BAD_PAGE;
-            }
-            const uint32_t there = __ballot_sync(0xffffffffu, at >= 0) & 0xFFFFu;
-            if (lane == 0) masks[warp][stage] = there;
-            const uint32_t kd = ring + stage * 2 * TILE, vd = kd + TILE;
             const int c = lane % CHUNKS;
 #pragma unroll
             for (int r0 = 0; r0 < SH_KEYS; r0 += PASS) {
                 const int r = r0 + lane / CHUNKS;
                 const int64_t row = __shfl_sync(0xffffffffu, at, r);
-                const int64_t off = row < 0 ? 0 : row + c * 8;
-                sh_copy16(kd + (r * LD + c * 8) * 2, p.k_pool + off, row >= 0);
-                sh_copy16(vd + (r * LD + c * 8) * 2, p.v_pool + off, row >= 0);
+                sh_copy16(dst + (r * LD + c * 8) * 2, pool + (row < 0 ? 0 : row + c * 8), row >= 0);
             }
         }
         ns_cp_commit();
     };
-    float acc[DH / 8][4];
+    auto note = [&](int stage, int64_t at) {
+        const uint32_t there = __ballot_sync(0xffffffffu, at >= 0) & 0xFFFFu;
+        if (lane == 0) masks[warp][stage] = there;
+    };
+    int64_t ahead = -1;                                // of the tile after next: its keys' rows
+    int page = -1;                                     // and of the one behind that: its pages, which nothing waits for yet
+    int pages[SH_STAGES];
 #pragma unroll
-    for (int n = 0; n < DH / 8; n++)
+    for (int s = 0; s < SH_STAGES; s++) pages[s] = page_of(t0 + warp + s * SH_WARPS);
+    page = page_of(t0 + warp + SH_STAGES * SH_WARPS);
 #pragma unroll
-        for (int e = 0; e < 4; e++) acc[n][e] = 0.0f;
-    float m[2] = {-INFINITY, -INFINITY}, l[2] = {0.0f, 0.0f};
+    for (int s = 0; s < SH_STAGES; s++) {
+        const int t = t0 + warp + s * SH_WARPS;
+        ahead = locate(t, pages[s]);
+        note(s, ahead);
+        load(t, ring + s * 2 * TILE, p.k_pool, ahead);
+        load(t, ring + s * 2 * TILE + TILE, p.v_pool, ahead);
+    }
+
+    // ---- queries: B fragments
+    uint32_t qf[DH / 16][2 * NT];
 #pragma unroll
-    for (int s = 0; s < SH_STAGES - 1; s++) load(t0 + warp + s * SH_WARPS, s);
+    for (int n = 0; n < NT; n++) {
+        const int r = row0 + n * 8 + fg, token = r / p.group;
+        const uint16_t* q = p.q + (int64_t)token * p.q_stride + (int64_t)(kvh * p.group + r - token * p.group) * DH + ft * 2;
+#pragma unroll
+        for (int kk = 0; kk < DH / 16; kk++)
+#pragma unroll
+            for (int e = 0; e < 2; e++) qf[kk][2 * n + e] = r < row_end ? *reinterpret_cast<const uint32_t*>(q + kk * 16 + e * 8) : 0u;
+    }
+    float acc[DH / 16][4 * NT];
+#pragma unroll
+    for (int n = 0; n < DH / 16; n++)
+#pragma unroll
+        for (int e = 0; e < 4 * NT; e++) acc[n][e] = 0.0f;
+    float m[2 * NT], l[2 * NT];                        // of rows 2 t and 2 t + 1 of each 8
+#pragma unroll
+    for (int e = 0; e < 2 * NT; e++) {
+        m[e] = -INFINITY;
+        l[e] = 0.0f;
+    }
     int stage = 0;
     for (int t = t0 + warp; t < t1; t += SH_WARPS) {
-        ns_cp_wait<SH_STAGES - 2>();
-        __syncwarp();
         const uint32_t kt = ring + stage * 2 * TILE, vt = kt + TILE;
+        // in order: K and V of this tile, K and V of the next
+        ns_cp_wait<2 * SH_STAGES - 1>();
+        __syncwarp();
         const uint32_t there = masks[warp][stage];
-        load(t + (SH_STAGES - 1) * SH_WARPS, stage == 0 ? SH_STAGES - 1 : stage - 1);
-        float s[2][4] = {{0.0f, 0.0f, 0.0f, 0.0f}, {0.0f, 0.0f, 0.0f, 0.0f}};
+        float s[4 * NT];
+#pragma unroll
+        for (int e = 0; e < 4 * NT; e++) s[e] = 0.0f;
 #pragma unroll
         for (int kk = 0; kk < DH / 16; kk++) {
-            uint32_t kb[4];
-            ns_ldsm4(kb, ns_addr_b(kt, LD, 0, kk * 16, lane));
-            ns_mma_bf16(s[0], qf[kk], kb[0], kb[1]);
-            ns_mma_bf16(s[1], qf[kk], kb[2], kb[3]);
+            uint32_t ka[4];
+            ns_ldsm4(ka, ns_addr_a(kt, LD, 0, kk * 16, lane));
+#pragma unroll
+            for (int n = 0; n < NT; n++) ns_mma_bf16(*reinterpret_cast<float(*)[4]>(&s[4 * n]), ka, qf[kk][2 * n], qf[kk][2 * n + 1]);
         }
-        float mx[2] = {-INFINITY, -INFINITY};
-#pragma unroll
-        for (int n = 0; n < 2; n++)
-#pragma unroll
-            for (int e = 0; e < 4; e++) {
-                const int c = n * 8 + fc + (e & 1);
-                const bool live = ((there >> c) & 1u) != 0 && t * SH_KEYS + c < limit[e >> 1];
-                s[n][e] = live ? s[n][e] * p.scale_log2 : -INFINITY;
-                mx[e >> 1] = fmaxf(mx[e >> 1], s[n][e]);
-            }
+        __syncwarp();
+        const int next = t + SH_STAGES * SH_WARPS;
+        ahead = locate(next, page);
+        page = page_of(next + SH_WARPS);
+        note(stage, ahead);
+        load(next, kt, p.k_pool, ahead);
+        // s[4 n + 2 h + e]: key g + 8 h, row 2 t + e of the n-th 8
+        float mx[2 * NT];
         bool grew = false;
 #pragma unroll
-        for (int h = 0; h < 2; h++) {
-            mx[h] = fmaxf(mx[h], __shfl_xor_sync(0xffffffffu, mx[h], 1));
-            mx[h] = fmaxf(mx[h], __shfl_xor_sync(0xffffffffu, mx[h], 2));
-            grew |= mx[h] > m[h];
+        for (int i = 0; i < 2 * NT; i++) {
+            const int n = i >> 1, e = i & 1;
+#pragma unroll
+            for (int h = 0; h < 2; h++) {
+                const int c = fg + 8 * h;
+                const bool live = ((there >> c) & 1u) != 0 && t * SH_KEYS + c < limit[i];
+                s[4 * n + 2 * h + e] = live ? s[4 * n + 2 * h + e] * p.scale_log2 : -INFINITY;
+            }
+            mx[i] = fmaxf(s[4 * n + e], s[4 * n + 2 + e]);
+#pragma unroll
+            for (int o = 4; o < 32; o <<= 1) mx[i] = fmaxf(mx[i], __shfl_xor_sync(0xffffffffu, mx[i], o));
+            grew |= mx[i] > m[i];
         }
         if (__any_sync(0xffffffffu, grew)) {
 #pragma unroll
-            for (int h = 0; h < 2; h++) {
-                const float up = fmaxf(m[h], mx[h]), f = m[h] == up ? 1.0f : ns_exp2(m[h] - up);
-                m[h] = up;
-                l[h] *= f;
+            for (int i = 0; i < 2 * NT; i++) {
+                const float up = fmaxf(m[i], mx[i]), f = m[i] == up ? 1.0f : ns_exp2(m[i] - up);
+                m[i] = up;
+                l[i] *= f;
 #pragma unroll
-                for (int n = 0; n < DH / 8; n++) {
-                    acc[n][2 * h] *= f;
-                    acc[n][2 * h + 1] *= f;
+                for (int d = 0; d < DH / 16; d++) {
+                    acc[d][4 * (i >> 1) + (i & 1)] *= f;
+                    acc[d][4 * (i >> 1) + 2 + (i & 1)] *= f;
                 }
             }
         }
-        uint32_t hi[4], lo[4];
+        uint32_t hi[2 * NT], lo[2 * NT];
 #pragma unroll
-        for (int n = 0; n < 2; n++)
+        for (int n = 0; n < NT; n++)
 #pragma unroll
             for (int h = 0; h < 2; h++) {
                 // (nothing seen yet: the scores are -infinity, their weights 0)
-                const float base = m[h] == -INFINITY ? 0.0f : m[h];
-                const float e0 = ns_exp2(s[n][2 * h] - base), e1 = ns_exp2(s[n][2 * h + 1] - base);
-                l[h] += e0 + e1;
+                const float b0 = m[2 * n] == -INFINITY ? 0.0f : m[2 * n], b1 = m[2 * n + 1] == -INFINITY ? 0.0f : m[2 * n + 1];
+                const float e0 = ns_exp2(s[4 * n + 2 * h] - b0), e1 = ns_exp2(s[4 * n + 2 * h + 1] - b1);
+                l[2 * n] += e0;
+                l[2 * n + 1] += e1;
                 const uint32_t w = ns_pack_bf16x2(e0, e1);
-                hi[2 * n + h] = w;
-                lo[2 * n + h] = ns_pack_bf16x2(e0 - __uint_as_float(w << 16), e1 - __uint_as_float(w & 0xFFFF0000u));
+                hi[2 * n + h] = sh_transpose(w);
+                lo[2 * n + h] = sh_transpose(ns_pack_bf16x2(e0 - __uint_as_float(w << 16), e1 - __uint_as_float(w & 0xFFFF0000u)));
             }
+        ns_cp_wait<2 * SH_STAGES - 1>();
+        __syncwarp();
 #pragma unroll
-        for (int n = 0; n < DH / 16; n++) {
-            uint32_t vb[4];
-            ns_ldsm4_t(vb, ns_addr_bt(vt, LD, 0, n * 16, lane));
-            ns_mma_bf16(acc[2 * n], hi, vb[0], vb[1]);
-            ns_mma_bf16(acc[2 * n + 1], hi, vb[2], vb[3]);
-            ns_mma_bf16(acc[2 * n], lo, vb[0], vb[1]);
-            ns_mma_bf16(acc[2 * n + 1], lo, vb[2], vb[3]);
+        for (int d = 0; d < DH / 16; d++) {
+            uint32_t va[4];
+            ns_ldsm4_t(va, ns_addr_at(vt, LD, d * 16, 0, lane));
+#pragma unroll
+            for (int n = 0; n < NT; n++) {
+                float(&a)[4] = *reinterpret_cast<float(*)[4]>(&acc[d][4 * n]);
+                ns_mma_bf16(a, va, hi[2 * n], hi[2 * n + 1]);
+                ns_mma_bf16(a, va, lo[2 * n], lo[2 * n + 1]);
+            }
         }
         __syncwarp();
+        load(next, vt, p.v_pool, ahead);
         stage = stage == SH_STAGES - 1 ? 0 : stage + 1;
     }
     ns_cp_wait<0>();
 
     // ---- the warps' results fold, in warp order
 #pragma unroll
-    for (int h = 0; h < 2; h++) {
-        l[h] += __shfl_xor_sync(0xffffffffu, l[h], 1);
-        l[h] += __shfl_xor_sync(0xffffffffu, l[h], 2);
-        if ((lane & 3) == 0) fold[warp][fr + 8 * h] = make_float2(m[h], l[h]);
+    for (int i = 0; i < 2 * NT; i++) {
+#pragma unroll
+        for (int o = 4; o < 32; o <<= 1) l[i] += __shfl_xor_sync(0xffffffffu, l[i], o);
+        if (fg == 0) fold[warp][(i >> 1) * 8 + ft * 2 + (i & 1)] = make_float2(m[i], l[i]);
     }
     __syncthreads();                      // every ring is free
-    float* out = reinterpret_cast<float*>(sh_smem) + warp * SH_ROWS * (DH + 4);
+    // acc[d][4 n + 2 h + e]: dimension 16 d + g + 8 h, row 2 t + e of the n-th 8
+    float* out = reinterpret_cast<float*>(sh_smem) + warp * ROWS * (DH + 4);
 #pragma unroll
-    for (int n = 0; n < DH / 8; n++)
+    for (int d = 0; d < DH / 16; d++)
 #pragma unroll
-        for (int h = 0; h < 2; h++)
-            *reinterpret_cast<float2*>(out + (fr + 8 * h) * (DH + 4) + n * 8 + fc) = make_float2(acc[n][2 * h], acc[n][2 * h + 1]);
+        for (int e = 0; e < 4 * NT; e++) out[((e >> 2) * 8 + ft * 2 + (e & 1)) * (DH + 4) + d * 16 + fg + ((e >> 1) & 1) * 8] = acc[d][e];
     __syncthreads();
     const bool alone = p.part_o == nullptr;
-    for (int e = threadIdx.x; e < SH_ROWS * DH; e += SH_THREADS) {
+    for (int e = threadIdx.x; e < ROWS * DH; e += SH_THREADS) {
         const int rr = e / DH, c = e % DH, r = row0 + rr;
         if (r >= row_end) break;
         float M = -INFINITY;
@@ -240,7 +284,7 @@ __global__ void __launch_bounds__(SH_THREADS, 3) ns_attention_shared_walk_kernel
             // (a warp that saw nothing has a sum of 0)
             const float f = fold[w][rr].x == -INFINITY ? (fold[w][rr].y == 0.0f ? 0.0f : 1.0f) : ns_exp2(fold[w][rr].x - M);
             L = fmaf(fold[w][rr].y, f, L);
-            O = fmaf(reinterpret_cast<float*>(sh_smem)[(w * SH_ROWS + rr) * (DH + 4) + c], f, O);
+            O = fmaf(reinterpret_cast<float*>(sh_smem)[(w * ROWS + rr) * (DH + 4) + c], f, O);
         }
         if (alone) {
             const int token = r / p.group, i = token % p.steps;
@@ -250,6 +294,16 @@ __global__ void __launch_bounds__(SH_THREADS, 3) ns_attention_shared_walk_kernel
             const int64_t at = ((int64_t)part * p.kv_heads + kvh) * rows_all + r;
             p.part_o[at * DH + c] = O;
             if (c == 0) p.part_ml[at] = make_float2(M, L);
+        }
+    }
+    // The kernel that folds follows this one alone: the last CTA to get here waits for the other kernel.  (Were each to wait, those to come would find no room.)
+    if (p.beside != nullptr) {
+        __shared__ int last;
+        if (threadIdx.x == 0) last = atomicAdd(p.beside, 1u) == gridDim.x - 1 ? 1 : 0;
+        __syncthreads();
+        if (last != 0) {
+            if (threadIdx.x == 0) *p.beside = 0;
+            ns_pdl_wait();
         }
     }
 }
@@ -318,17 +372,26 @@ __global__ void __launch_bounds__(256) ns_attention_shared_fold_kernel(const Sha
     for (int n = 0; n < N; n++) dst[n] = ns_f32_to_bf16_bits(L == 0.0f ? 0.0f : O[n] * inv);
 }
 
-template <int DH>
-int launch_shared(NsDevice* d, const SharedParams& p)
+template <int DH, int NT>
+int launch_walk(NsDevice* d, const SharedParams& p, int64_t ctas)
 {
     constexpr int smem = SH_WARPS * SH_STAGES * 2 * SH_KEYS * (DH + 8) * 2;
-    static_assert(smem >= SH_WARPS * SH_ROWS * (DH + 4) * 4, "the fold's rows");
+    static_assert(smem >= SH_WARPS * 8 * NT * (DH + 4) * 4, "the fold's rows");
+    auto walk = ns_attention_shared_walk_kernel<DH, NT>;
+    NS_CUDA(cudaFuncSetAttribute(walk, cudaFuncAttributeMaxDynamicSharedMemorySize, smem));
+    if (p.beside != nullptr) NS_CUDA(ns_launch_pdl(walk, dim3((unsigned)ctas), dim3(SH_THREADS), smem, d->stream, p));
+    else NS_CUDA(ns_launch_plain(walk, dim3((unsigned)ctas), dim3(SH_THREADS), smem, d->stream, p));
+    return NS_OK;
+}
+
+template <int DH>
+int launch_shared(NsDevice* d, const SharedParams& p, int row_tile)
+{
     const int64_t ctas = (int64_t)p.kv_heads * ((int64_t)p.prefix_tiles * p.prefix_parts + (int64_t)p.batch * p.own_tiles * p.own_parts);
     NS_REQUIRE(ctas < (1LL << 31), NS_ERR_ARGUMENT, "ns_attention_shared: too many rows");
     if (ctas > 0) {
-        auto walk = ns_attention_shared_walk_kernel<DH>;
-        NS_CUDA(cudaFuncSetAttribute(walk, cudaFuncAttributeMaxDynamicSharedMemorySize, smem));
-        NS_CUDA(ns_launch_plain(walk, dim3((unsigned)ctas), dim3(SH_THREADS), smem, d->stream, p));
+        const int rc = row_tile == 8 ? launch_walk<DH, 1>(d, p, ctas) : launch_walk<DH, 2>(d, p, ctas);
+        if (rc != NS_OK) return rc;
     }
     if (p.part_o != nullptr) {
         const int64_t rows = (int64_t)p.batch * p.steps * p.heads;
@@ -378,6 +441,7 @@ extern "C" int ns_attention_shared(ns_device_t h, ns_kv_cache_t cache, uint64_t 
     p.batch = batch; p.steps = steps; p.heads = heads; p.kv_heads = c.heads; p.group = heads / c.heads;
     p.scale_log2 = scale * 1.4426950408889634f;
     p.status = d->status_dev;
+    p.beside = nullptr;
     const int64_t rows = (int64_t)batch * steps * p.group;
     // parts by position: until there are about four CTAs an SM, 64 keys a part at least
     auto parts = [&](int64_t ctas, int64_t positions) {
@@ -385,13 +449,15 @@ extern "C" int ns_attention_shared(ns_device_t h, ns_kv_cache_t cache, uint64_t 
         if (n > (positions + 63) / 64) n = (positions + 63) / 64;
         return (int)(n < 1 ? 1 : n > 64 ? 64 : n);
     };
+    // rows of a CTA of the walking kernel: those of one token, or of all, where they fit into 8
+    const int row_tile = steps * p.group <= 8 ? 8 : 16;
     p.prefix_tiles = 0;
     const bool tiles = ns_attention_shared_tiles_fit(d, p, c.head_dim, scale, &p.prefix_parts);
     if (!tiles) {
-        p.prefix_tiles = (int)((rows + SH_ROWS - 1) / SH_ROWS);
+        p.prefix_tiles = (int)((rows + row_tile - 1) / row_tile);
         p.prefix_parts = prefix_pages == 0 ? 0 : parts((int64_t)p.prefix_tiles * c.heads, (int64_t)prefix_pages * c.page_size);
     }
-    p.own_tiles = (steps * p.group + SH_ROWS - 1) / SH_ROWS;
+    p.own_tiles = (steps * p.group + row_tile - 1) / row_tile;
     p.own_parts = max_pages == 0 ? 0 : parts((int64_t)batch * p.own_tiles * c.heads, (int64_t)max_pages * c.page_size);
     const int n_parts = p.prefix_parts + p.own_parts;
     p.part_o = nullptr;
@@ -405,12 +471,13 @@ extern "C" int ns_attention_shared(ns_device_t h, ns_kv_cache_t cache, uint64_t 
         p.part_ml = reinterpret_cast<float2*>(p.part_o + sums * c.head_dim);
     }
     if (tiles) {
+        if (ns_pdl_enabled()) p.beside = d->sync_words + NS_SYNC_BESIDE;
         rc = ns_attention_shared_tiles(d, p, c.head_dim);
         if (rc != NS_OK) return rc;
     }
     switch (c.head_dim) {
-        case 32: return launch_shared<32>(d, p);
-        case 64: return launch_shared<64>(d, p);
-        default: return launch_shared<128>(d, p);
+        case 32: return launch_shared<32>(d, p, row_tile);
+        case 64: return launch_shared<64>(d, p, row_tile);
+        default: return launch_shared<128>(d, p, row_tile);
     }
 }

@@ -25,6 +25,7 @@ struct SharedParams {
     float* part_o;                         // [parts, kv_heads, rows, head_dim]: weighted values relative to the part's maximum
     float2* part_ml;                       // [parts, kv_heads, rows]: maximum in units of log2, sum; (-infinity, 0): nothing seen, and no values written
     int* status;
+    uint32_t* beside;                      // the walking kernel runs beside the tensor-core kernel: a word that counts its CTAs, zero between kernels
 };
 
 // Whether the tensor-core kernel can read the prefix of such a cache, and its number of parts; ns_attention_shared_tiles queues it.

@@ -37,9 +37,9 @@ int ns_fail(int code, const char* fmt, ...);  // records the message, returns co
 
 // Slots of the device status block kernels write to when a bounded wait gives up.
 enum { NS_STATUS_WORDS = 16 };
-// Device words for grid-wide phases: [0] arrivals, [1] departures of the product kernels' second phase;
+// Device words for grid-wide phases: [0] arrivals, [1] departures of the product kernels' second phase; [NS_SYNC_BESIDE] finished CTAs of a kernel beside another;
 // [NS_SYNC_ROW_TICKETS, +NS_SYNC_MAX_ROWS) one ticket per activation row for the decode attention's row quantisation.
-enum { NS_SYNC_WORDS = 4096, NS_SYNC_ROW_TICKETS = 64, NS_SYNC_MAX_ROWS = 4000 };
+enum { NS_SYNC_WORDS = 4096, NS_SYNC_BESIDE = 2, NS_SYNC_ROW_TICKETS = 64, NS_SYNC_MAX_ROWS = 4000 };
 
 struct NsDevice {
     int ordinal = 0;
