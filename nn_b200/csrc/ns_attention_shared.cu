@@ -471,7 +471,7 @@ extern "C" int ns_attention_shared(ns_device_t h, ns_kv_cache_t cache, uint64_t 
         p.part_ml = reinterpret_cast<float2*>(p.part_o + sums * c.head_dim);
     }
     if (tiles) {
-        if (ns_pdl_enabled()) p.beside = d->sync_words + NS_SYNC_BESIDE;
+        if (ns_pdl_enabled() && max_pages > 0) p.beside = d->sync_words + NS_SYNC_BESIDE;
         rc = ns_attention_shared_tiles(d, p, c.head_dim);
         if (rc != NS_OK) return rc;
     }

@@ -23,6 +23,7 @@ namespace {
 
 constexpr int ST_THREADS = 384;
 constexpr int ST_KB = 128;                             // keys a block
+constexpr int ST_OWN = 300;                            // own positions of a key/value head that are as much work as a unit
 constexpr int ST_EARLY = 4;                            // blocks in which every growth of the maximum is followed
 constexpr uint32_t ST_STAGE_BYTES = 32 * 128;          // a softmax warp's 32 rows x 32 floats on their way out
 constexpr uint32_t ST_S_COL = 128;                     // tensor memory of group g: O at columns 256 g, S 128 further on, P over the first half of S
@@ -61,6 +62,7 @@ struct TileParams {
     int turns;           // the groups own the same rows and take turns with the blocks
     int box;             // rows of a TMA box: a page, or 128 of it
     int parts;           // of a tile, at most (each two where the groups take turns)
+    int sms;
 };
 struct TileMaps {
     CUtensorMap k, v;    // [64 columns, box rows] of (columns, page rows, heads, pages)
@@ -76,11 +78,16 @@ struct Share {
     int blocks;          // of a tile
     int64_t at, end, total;
     int ctas;
-    __device__ __forceinline__ Share(const TileParams& p, int n_keys)
+    // own: positions that the walking kernel has to read beside this one.  The SMs are divided between the two in proportion to their work, a unit being as much as 300
+    // positions of a key/value head: the CTAs behind `most` leave, and the other kernel's take their place.  (256 sequences of 300 positions over 16384, 148 CTAs 141 us,
+    // 88 129; 64 of 257 over 4096, 128 CTAs 42.6, 57 35.6.)
+    __device__ __forceinline__ Share(const TileParams& p, int n_keys, float own)
     {
         blocks = (n_keys + ST_KB - 1) / ST_KB;
         total = (int64_t)blocks * p.tiles * p.s.kv_heads;
-        ctas = (int)(total < gridDim.x ? total : gridDim.x);       // no share is empty but behind these
+        const float units = (float)total * (p.turns ? 0.6f : 1.0f), beside = p.s.beside != nullptr ? own * (float)p.s.kv_heads * (1.0f / ST_OWN) : 0.0f;
+        const int most = min((int)gridDim.x, max(1, (int)((float)p.sms * units / (units + beside) + 0.5f)));
+        ctas = (int)(total < most ? total : most);                 // no share is empty but behind these
         at = end = 0;
         if ((int)blockIdx.x < ctas) {
             at = total * blockIdx.x / ctas;
@@ -199,6 +206,16 @@ __global__ void __launch_bounds__(ST_THREADS, 1) ns_attention_shared_tile_kernel
     const uint32_t tmem_slot = bar(L::COUNT);
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
 
+    __shared__ uint32_t own_sums[ST_THREADS / 32];
+    ns_pdl_wait();
+    ns_pdl_trigger();
+    // ---- this CTA's share, before anything else: the SMs of CTAs without one are the other kernel's
+    const int n_keys = sh_clamp(p.s.prefix_len[0], p.s.prefix_pages, p.s.page_shift);
+    uint32_t own = 0;                          // positions beside this kernel's, 16 at a time
+    if (p.s.beside != nullptr)
+        for (int b = threadIdx.x; b < p.s.batch; b += ST_THREADS) own = min(own + (uint32_t)(sh_clamp((int64_t)p.s.pos[b] + p.s.steps, p.s.max_pages, p.s.page_shift) >> 4), 1u << 26);
+    own = __reduce_add_sync(0xffffffffu, own);
+    if (lane == 0) own_sums[warp] = own;
     if (threadIdx.x == 0) {
         abort_flag_storage = 0;
         for (int i = 0; i < 2; i++) {
@@ -220,6 +237,13 @@ __global__ void __launch_bounds__(ST_THREADS, 1) ns_attention_shared_tile_kernel
         ns_prefetch_tensormap(&maps.v);
         ns_prefetch_tensormap(&maps.o);
     }
+    __syncthreads();
+    float own_all = 0.0f;
+#pragma unroll
+    for (int w = 0; w < ST_THREADS / 32; w++) own_all += (float)own_sums[w];
+    Share share(p, n_keys, 16.0f * own_all);
+    Item t;
+    if (share.at >= share.end && share.total != 0) return;
     if (warp == 1) {
         ns_tmem_alloc(tmem_slot, 512);
         ns_tmem_relinquish();
@@ -230,15 +254,10 @@ __global__ void __launch_bounds__(ST_THREADS, 1) ns_attention_shared_tile_kernel
     uint32_t tmem_base;
     asm volatile("ld.shared.b32 %0, [%1];" : "=r"(tmem_base) : "r"(tmem_slot));
     tmem_base = __shfl_sync(0xffffffffu, tmem_base, 0);
-    ns_pdl_wait();
-    ns_pdl_trigger();
-    const int n_keys = sh_clamp(p.s.prefix_len[0], p.s.prefix_pages, p.s.page_shift);
     const int code = 330;
     auto wait = [&](int i, uint32_t parity, int what) { return ns_mbar_wait_warp(bar(i), parity & 1u, abort_flag, p.s.status, code + what); };
     // whether group g has rows in a tile
     auto has_rows = [&](int g, const Item& t) { return p.turns != 0 || t.tile * 256 + 128 * g < p.rows; };
-    Share share(p, n_keys);
-    Item t;
     // the page of box `lane` of a block: -1 behind the prefix
     const int boxes = ST_KB / p.box, shift = p.s.page_shift;
     auto box_page = [&](int j) {
@@ -571,6 +590,7 @@ int tile_ctas(const NsDevice* d, const TileParams& p)
 void tile_plan(const NsDevice* d, const SharedParams& s, TileParams& p)
 {
     p.s = s;
+    p.sms = d->sm_count;
     p.rows = s.batch * s.steps * s.group;
     p.group.by(s.group);
     p.turns = p.rows <= 128 ? 1 : 0;
@@ -609,8 +629,11 @@ int launch_tiles(NsDevice* d, const TileParams& p)
 bool ns_attention_shared_tiles_fit(const NsDevice* d, const SharedParams& s, int head_dim, float scale, int* parts)
 {
     // boxes of fewer than 8 rows would not begin on the swizzle's 1 KB; the reference maximum is one of raw scores, so their order has to be that of
-    // the scaled ones; tensor maps count pages and rows in 32 bits
+    // the scaled ones
     if (head_dim < 64 || s.page_shift < 3 || !(scale > 0.0f) || s.prefix_pages == 0) return false;
+    // Little to multiply is the walking kernel's: it starts at once, this one needs some 12 us for its first results.  Both sides (us, this and the other): 64 query rows x 8 heads x
+    // 2000 keys x 128 22.5, 22.1; 32 x 8 x 8000 28.5, 31.8; 128 x 8 x 2000 22.9, 29.0; 512 x 8 x 500 40.5, 38.2; 64 columns: 128 x 8 x 2000 20.5, 20.8; 32 x 8 x 8000 27.6, 22.9; 64 x 8 x 8000 28.5, 30.4.
+    if ((double)s.batch * s.steps * s.heads * ((double)s.prefix_pages * (1 << s.page_shift)) * head_dim < 1.2e6 * 128) return false;
     TileParams p;
     tile_plan(d, s, p);
     *parts = p.parts * (p.turns ? 2 : 1);
