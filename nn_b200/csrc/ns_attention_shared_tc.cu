@@ -631,9 +631,11 @@ bool ns_attention_shared_tiles_fit(const NsDevice* d, const SharedParams& s, int
     // boxes of fewer than 8 rows would not begin on the swizzle's 1 KB; the reference maximum is one of raw scores, so their order has to be that of
     // the scaled ones
     if (head_dim < 64 || s.page_shift < 3 || !(scale > 0.0f) || s.prefix_pages == 0) return false;
-    // Little to multiply is the walking kernel's: it starts at once, this one needs some 12 us for its first results.  Both sides (us, this and the other): 64 query rows x 8 heads x
-    // 2000 keys x 128 22.5, 22.1; 32 x 8 x 8000 28.5, 31.8; 128 x 8 x 2000 22.9, 29.0; 512 x 8 x 500 40.5, 38.2; 64 columns: 128 x 8 x 2000 20.5, 20.8; 32 x 8 x 8000 27.6, 22.9; 64 x 8 x 8000 28.5, 30.4.
-    if ((double)s.batch * s.steps * s.heads * ((double)s.prefix_pages * (1 << s.page_shift)) * head_dim < 1.2e6 * 128) return false;
+    // Little to multiply is the walking kernel's, which starts at once; so is what few rows have to read of long keys, which it has on their way from more places.  Both sides of the
+    // line, us, this kernel's way and the other's (rows of a key/value head x heads x keys x columns): 32 x 8 x 2000 x 128 15.2, 16.0; 64 x 2 x 8000 x 128 19.5, 21.2; 128 x 8 x 2000 x 128 20.7,
+    // 28.6; 64 x 8 x 2000 x 64 14.2, 14.9; 64 x 1 x 8000 x 128 15.9, 15.7; 256 x 2 x 2000 x 64 16.9, 14.9; 8 x 8 x 8000 x 128 23.7, 15.8; 16 x 16 x 8000 x 128 32.6, 30.2.
+    const double work = (double)s.batch * s.steps * s.heads * ((double)s.prefix_pages * (1 << s.page_shift)) * head_dim;
+    if (work < ((int64_t)s.batch * s.steps * s.group >= 24 ? 0.8e6 : 4e6) * 128) return false;
     TileParams p;
     tile_plan(d, s, p);
     *parts = p.parts * (p.turns ? 2 : 1);
