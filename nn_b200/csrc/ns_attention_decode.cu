@@ -617,6 +617,7 @@ int ns_kv_cache_view(ns_kv_cache_t ch, NsKvCacheView* out)
     NS_REQUIRE(c != nullptr && out != nullptr, NS_ERR_ARGUMENT, "cache is null");
     out->k_pool = c->k_pool; out->v_pool = c->v_pool;
     out->page_size = c->page_size; out->heads = c->heads; out->head_dim = c->head_dim; out->num_pages = c->num_pages;
+    out->ordinal = c->ordinal;
     return NS_OK;
 }
 

@@ -455,6 +455,7 @@ extern "C" int ns_attention_shared(ns_device_t h, ns_kv_cache_t cache, uint64_t 
     NsDevice* d = ns_dev(h);
     rc = ns_device_make_current(d);
     if (rc != NS_OK) return rc;
+    NS_REQUIRE(c.ordinal == d->ordinal, NS_ERR_ARGUMENT, "ns_attention_shared: the cache is another device's");
     if (batch == 0 || steps == 0) return NS_OK;
     SharedParams p;
     p.q = reinterpret_cast<const uint16_t*>(q); p.q_stride = q_stride;

@@ -559,6 +559,7 @@ extern "C" int ns_kv_append_rotary(ns_device_t h, ns_kv_cache_t cache, uint64_t 
     NsDevice* d = ns_dev(h);
     rc = ns_device_make_current(d);
     if (rc != NS_OK) return rc;
+    NS_REQUIRE(c.ordinal == d->ordinal, NS_ERR_ARGUMENT, "ns_kv_append_rotary: the cache is another device's");
     const int rows = batch * steps;
     if (rows == 0) return NS_OK;
     AppendArgs p;

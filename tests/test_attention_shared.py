@@ -125,13 +125,22 @@ CASES = [  # dim, kv heads, group, page, prefix, own positions of each sequence 
     (32, 1, 40, 16, 200, [20, 25], 1),              # groups of more heads than a tile has rows
     (128, 1, 2, 256, 900, [300, 20], 70),           # a portion of a prompt
     (64, 2, 3, 64, 3000, [90] * 50, 1),
+    # work enough for the tensor-core kernel: 800 000 products of 128 columns
+    (128, 1, 8, 64, 2000, [40, 1] * 32, 1),         # 512 rows: two tiles
+    (128, 2, 4, 16, 3333, [17] * 32, 1),            # 128 rows: the groups take turns
+    (128, 4, 2, 8, 2600, [5, 60] * 20, 1),          # 80 rows
+    (64, 2, 8, 32, 4097, [33] * 33, 1),             # 264 rows: a group without rows
+    (64, 8, 1, 128, 5000, [9, 200] * 16, 2),        # 64 rows, two tokens each
+    (128, 1, 3, 256, 1153, [70] * 60, 5),           # 900 rows in groups of three
+    (128, 1, 12, 64, 129, [1] * 600, 1),            # 7200 rows, two blocks
+    (64, 1, 8, 16, 300, [] , 1),                    # (filled in below: many sequences without pages of their own)
 ]
 
 
 @pytest.mark.gpu
 @pytest.mark.parametrize("dim,kv,group,page,prefix,own,steps", CASES)
 def test_outputs(dev, dim, kv, group, page, prefix, own, steps):
-    s = Setup(dev, dim, kv, group, page, len(own) or 6, steps, prefix, own)
+    s = Setup(dev, dim, kv, group, page, len(own) or (700 if prefix == 300 else 6), steps, prefix, own)
     if not own:
         s.pos = np.zeros(s.batch, np.int32)
     s.upload()
@@ -143,7 +152,7 @@ def test_outputs(dev, dim, kv, group, page, prefix, own, steps):
 @pytest.mark.parametrize("dim,page,batch", [(128, 64, 3), (64, 16, 40), (32, 8, 3), (128, 16, 70), (64, 4, 5)])
 def test_padding_and_rows_that_see_nothing(dev, dim, page, batch):
     """Padded rows stay as they are; negative positions leave the prefix, without one zeros; positions beyond a table do not count; outputs with a gap."""
-    for prefix in (0, 75):
+    for prefix in (0, 75) if batch != 70 else (0, 1900):
         s = Setup(dev, dim, 2, 4, page, batch, 3, prefix, [41] * batch, seed=prefix)
         s.lens = s.rng.integers(0, 4, batch).astype(np.int32)
         s.pos = s.rng.integers(-4, 38, batch).astype(np.int32)
@@ -159,7 +168,8 @@ def test_padding_and_rows_that_see_nothing(dev, dim, page, batch):
 
 
 @pytest.mark.gpu
-@pytest.mark.parametrize("dim,kv,group,page,batch,prefix", [(128, 2, 4, 64, 5, 300), (64, 1, 2, 16, 3, 65), (32, 2, 4, 4, 4, 130), (128, 1, 4, 16, 64, 1000), (64, 1, 4, 32, 50, 77)])
+@pytest.mark.parametrize("dim,kv,group,page,batch,prefix", [(128, 2, 4, 64, 5, 300), (64, 1, 2, 16, 3, 65), (32, 2, 4, 4, 4, 130), (128, 1, 4, 16, 64, 1000), (64, 1, 4, 32, 50, 77),
+                                                              (128, 1, 8, 16, 64, 1700), (64, 2, 8, 64, 40, 3001), (128, 2, 4, 64, 16, 6500), (128, 1, 8, 256, 60, 2050)])
 def test_what_is_not_seen_does_not_count(dev, dim, kv, group, page, batch, prefix):
     """Behind the last position of the prefix and of every sequence, and in pages nobody names: NaN, infinities, the type's lowest value."""
     own = [1 + (7 * b) % 45 for b in range(batch)]
@@ -180,12 +190,12 @@ def test_what_is_not_seen_does_not_count(dev, dim, kv, group, page, batch, prefi
 
 
 @pytest.mark.gpu
-@pytest.mark.parametrize("dim,page,batch", [(128, 64, 2), (64, 16, 40), (128, 16, 70), (32, 16, 5)])
-def test_scores_that_are_no_numbers(dev, dim, page, batch):
+@pytest.mark.parametrize("dim,page,batch,prefix", [(128, 64, 2, 200), (64, 16, 40, 200), (128, 16, 70, 200), (32, 16, 5, 200), (128, 16, 70, 3000), (64, 64, 30, 14000)])
+def test_scores_that_are_no_numbers(dev, dim, page, batch, prefix):
     """A NaN among the keys a row sees makes the row NaN, and only the rows that see it; a value of NaN too."""
     for where in ("prefix", "own"):
         for what in "kv":
-            s = Setup(dev, dim, 1, 4, page, batch, 1, 200, [50] * batch)
+            s = Setup(dev, dim, 1, 4, page, batch, 1, prefix, [50] * batch)
             table, j = (s.prefix_table, 130) if where == "prefix" else (s.table[1], 20)
             getattr(s, what)[table[j // page], 0, j % page, 3] = 0x7FC0
             s.upload()
@@ -199,7 +209,7 @@ def test_scores_that_are_no_numbers(dev, dim, page, batch):
 
 
 @pytest.mark.gpu
-@pytest.mark.parametrize("dim,page,batch,prefix", [(128, 16, 3, 100), (64, 64, 40, 500), (128, 32, 100, 1111), (32, 4, 4, 50)])
+@pytest.mark.parametrize("dim,page,batch,prefix", [(128, 16, 3, 100), (64, 64, 40, 500), (128, 32, 100, 1111), (32, 4, 4, 50), (128, 16, 40, 2600), (64, 8, 150, 1500), (128, 128, 64, 1600)])
 def test_pages_outside_the_pool(dev, dim, page, batch, prefix):
     """Positions of a page that is none are left out and reported."""
     s = Setup(dev, dim, 2, 4, page, batch, 1, prefix, [60] * batch)
@@ -228,10 +238,10 @@ def test_pages_outside_the_pool(dev, dim, page, batch, prefix):
 
 
 @pytest.mark.gpu
-@pytest.mark.parametrize("dim,group,batch", [(128, 4, 40), (64, 1, 3)])
-def test_values_alike(dev, dim, group, batch):
+@pytest.mark.parametrize("dim,group,batch,prefix", [(128, 4, 40, 900), (64, 1, 3, 900), (128, 4, 40, 6000), (64, 4, 100, 4100)])
+def test_values_alike(dev, dim, group, batch, prefix):
     """Weights add up to one: values that are all alike come back within the rounding of the weights and of the output."""
-    s = Setup(dev, dim, 1, group, 64, batch, 1, 900, [70] * batch)
+    s = Setup(dev, dim, 1, group, 64, batch, 1, prefix, [70] * batch)
     s.v[:] = bf16(np.broadcast_to(np.linspace(-3, 3, dim, dtype=np.float32), s.v.shape))[0]
     s.upload()
     got, want = values(s.call()).astype(np.float64), values(s.v[0, 0, 0]).astype(np.float64)
@@ -240,11 +250,11 @@ def test_values_alike(dev, dim, group, batch):
 
 
 @pytest.mark.gpu
-@pytest.mark.parametrize("batch", [2, 40])
-def test_a_pool_of_more_than_2_31_elements(dev, batch):
+@pytest.mark.parametrize("batch,prefix", [(2, 200), (40, 200), (20, 1300)])
+def test_a_pool_of_more_than_2_31_elements(dev, batch, prefix):
     dim, kv, page = 128, 8, 64
     n = 2 ** 31 // (kv * page * dim) + 200
-    s = Setup(dev, dim, kv, 4, page, batch, 1, 200, [70] * batch)
+    s = Setup(dev, dim, kv, 4, page, batch, 1, prefix, [70] * batch)
     N.call("ns_kv_cache_destroy", s.cache)
     s.cache = C.c_void_p()
     N.call("ns_kv_cache_create", dev.handle, n, page, kv, dim, C.byref(s.cache))
@@ -263,7 +273,8 @@ def test_a_pool_of_more_than_2_31_elements(dev, batch):
 @pytest.mark.gpu
 def test_replays_with_other_lengths(dev):
     """A recorded call follows the device's positions, length and tables; two recorded calls share the scratch block in stream order."""
-    sets = [Setup(dev, 128, 2, 4, 64, 6, 1, 500, [90] * 6, seed=1), Setup(dev, 64, 2, 4, 16, 40, 1, 300, [50] * 40, seed=2)]
+    sets = [Setup(dev, 128, 2, 4, 64, 6, 1, 500, [90] * 6, seed=1), Setup(dev, 64, 2, 4, 16, 40, 1, 300, [50] * 40, seed=2), Setup(dev, 128, 2, 4, 16, 48, 1, 2200, [50] * 48, seed=3),
+            Setup(dev, 64, 1, 8, 64, 70, 1, 3000, [80] * 70, seed=4)]
     graphs = []
     for s in sets:
         s.upload()
@@ -273,7 +284,7 @@ def test_replays_with_other_lengths(dev):
         dev.capture_begin()
         N.call("ns_attention_shared", *a)
         graphs.append(dev.capture_end())
-    for prefix, own in ((500, 90), (1, 1), (77, 30), (300, 50)):
+    for prefix, own in ((500, 90), (1, 1), (77, 30), (0, 3), (127, 9), (128, 9), (129, 50), (1025, 20), (9999, 50)):
         for s in sets:
             s.prefix, s.pos = min(prefix, s.prefix_pages * s.page), np.full(s.batch, min(own, s.max_pages * s.page) - 1, np.int32)
             s.kept[2].upload(np.array([s.prefix], np.int32))
@@ -291,7 +302,7 @@ def test_replays_with_other_lengths(dev):
 
 @pytest.mark.gpu
 def test_runs_repeat_bit_for_bit(dev):
-    for batch in (3, 64):
+    for batch in (3, 64, 20):
         s = Setup(dev, 128, 4, 4, 32, batch, 1, 3000, [200] * batch)
         s.upload()
         first = s.call()

@@ -1,8 +1,8 @@
 """ns_sample_tokens against its definition in 64 bits: sort, cut, draw.
 
-Tokens have to be the definition's: the kernel's sums are exact to 2^-44 of the largest weight, and a random number falls that close to a border once in some
-10^8 rows.  The probability is one rounding to 32 bits (half a step, 2^-24) of a quotient of sums that are each within vocabulary * 2^-45, relative to a sum that is one
-at least, and of a weight that is a multiple of 2^-44: 2^-24 of it and 2^-44 * vocabulary."""
+Tokens have to be the definition's: the kernel's weights are within 2^-33 of themselves and their sums exact, so a random number falls between the two sides' borders once in some
+10^6 rows of the largest vocabularies here.  The probability is one rounding to 32 bits (half a step, 2^-24) of a quotient of a weight and a sum of weights, each within
+2^-33, and every weight is rounded to a multiple of 2^-42 of the largest, half a step 2^-43: 2^-24 + 2^-32 of it, and 2^-42 * vocabulary."""
 import numpy as np
 import pytest
 
@@ -61,7 +61,7 @@ def check(ids, probs, x, s):
     for r in range(len(x)):
         i, p = define(x[r], get("temperature", r, 1.0), int(get("top_k", r, 0)), float(get("top_p", r, 1.0)), float(get("min_p", r, 0.0)), float(s["u"][r]))
         assert ids[r] == i, (r, ids[r], i, {n: a[r] for n, a in s.items() if a is not None})
-        assert abs(probs[r] - p) <= 2.0 ** -24 * p + 2.0 ** -44 * vocab, (r, probs[r], p)
+        assert abs(probs[r] - p) <= (2.0 ** -24 + 2.0 ** -32) * p + 2.0 ** -42 * vocab, (r, probs[r], p)
 
 
 # one CTA a row and clusters of 2, 4 and 8; vocabularies that fill no vector; rows in numbers that fill the machine or not
