@@ -28,13 +28,19 @@ constexpr int ST_EARLY = 4;                            // blocks in which every 
 constexpr uint32_t ST_STAGE_BYTES = 32 * 128;          // a softmax warp's 32 rows x 32 floats on their way out
 constexpr uint32_t ST_S_COL = 128;                     // tensor memory of group g: O at columns 256 g, S 128 further on, P over the first half of S
 
+// Rows of 128 bytes, 64 columns.  Heads of 32 columns lie two keys a row, key 2 i before key 2 i + 1 as they lie in the page: the first 64 scores are those of the even keys, the
+// products' operands the first 32 columns, and the other 64 those of the odd ones.
 template <int DH>
 struct Layout {
-    static constexpr int HALVES = DH / 64;                     // column blocks of 64, 128 bytes a row
+    static constexpr bool TWO = DH == 32;                      // keys a row
+    static constexpr int HALVES = DH == 128 ? 2 : 1;           // column blocks of 64
     static constexpr int SLOTS = DH == 128 ? 2 : 4;
-    static constexpr uint32_t HALF = ST_KB * 128;
+    static constexpr int KEYS = TWO ? 2 : 1;
+    static constexpr uint32_t HALF = ST_KB / KEYS * 128;
     static constexpr uint32_t KV = HALVES * HALF;
     static constexpr uint32_t Q = HALVES * 128 * 128;
+    // the key of a block's score c
+    static __device__ __forceinline__ constexpr int key(int c) { return TWO ? c % 64 * 2 + c / 64 : c; }
     static constexpr uint32_t K_AT = 2 * Q, V_AT = K_AT + SLOTS * KV, STAGE_AT = V_AT + SLOTS * KV, BAR_AT = STAGE_AT + 8 * ST_STAGE_BYTES;
     static constexpr uint32_t SMEM = 1024 + BAR_AT + 512;
     // barriers
@@ -280,7 +286,7 @@ __global__ void __launch_bounds__(ST_THREADS, 1) ns_attention_shared_tile_kernel
                 for (int j = t.b0; j < t.b1; j++, ring.next()) {
                     const int next = j + 1 < t.b1 ? box_page(j + 1) : -1;
                     if (__any_sync(0xffffffffu, box_bad(j, page)) && lane == 0) *reinterpret_cast<volatile int*>(p.s.status) = SH_BAD_PAGE;
-                    const int row = (j * ST_KB) & ((1 << shift) - 1);        // inside its page, where that is longer than a block
+                    const int row = ((j * ST_KB) & ((1 << shift) - 1)) / L::KEYS;        // inside its page, where that is longer than a block
                     // a page that is none reads as zeros: its coordinate lies behind the pool
                     const int at = page < 0 || page >= p.s.num_pages ? p.s.num_pages : page;
                     auto load = [&](const CUtensorMap* map, uint32_t dst, uint32_t full) {
@@ -289,7 +295,7 @@ __global__ void __launch_bounds__(ST_THREADS, 1) ns_attention_shared_tile_kernel
                             const int pg = __shfl_sync(0xffffffffu, at, i);
                             if (leader) {
 #pragma unroll
-                                for (int h = 0; h < L::HALVES; h++) ns_tma_load_4d(dst + h * L::HALF + i * p.box * 128, map, full, h * 64, row, t.kvh, pg);
+                                for (int h = 0; h < L::HALVES; h++) ns_tma_load_4d(dst + h * L::HALF + i * (p.box / L::KEYS) * 128, map, full, h * 64, row, t.kvh, pg);
                             }
                         }
                     };
@@ -314,10 +320,13 @@ __global__ void __launch_bounds__(ST_THREADS, 1) ns_attention_shared_tile_kernel
                         load(&maps.v, v, bar(L::V_TAIL));
                         ok = wait(L::V_TAIL, tails++, 3);
                         if (!ok) break;
-                        for (int e = lane; e < (ST_KB - live) * 8 * L::HALVES; e += 32) {
-                            const int c = e & 7, r = live + (e >> 3) % (ST_KB - live), h = (e >> 3) / (ST_KB - live);
+                        const int rows = (live + L::KEYS - 1) / L::KEYS, gone = ST_KB / L::KEYS - rows;
+                        for (int e = lane; e < gone * 8 * L::HALVES; e += 32) {
+                            const int c = e & 7, r = rows + (e >> 3) % gone, h = (e >> 3) / gone;
                             ns_st_shared_v4(v + h * L::HALF + r * 128 + c * 16, 0, 0, 0, 0);
                         }
+                        // (the second key of a row: its pieces 4 to 7, where the swizzle puts them)
+                        if (L::TWO && (live & 1) != 0 && lane < 4) ns_st_shared_v4(v + (rows - 1) * 128 + (((4 + lane) ^ ((rows - 1) & 7)) * 16), 0, 0, 0, 0);
                         ns_fence_proxy_async();
                         __syncwarp();
                         if (leader) ns_mbar_arrive(bar(L::V_FULL + ring.s));
@@ -328,7 +337,7 @@ __global__ void __launch_bounds__(ST_THREADS, 1) ns_attention_shared_tile_kernel
         } else if (warp == 1) {
             // ------------------------------------------------------------ MMAs
             const bool leader = ns_elect();
-            constexpr uint32_t idesc_qk = ns_idesc(1, 1, 0, 0, 128, ST_KB), idesc_pv = ns_idesc(1, 1, 0, 1, 128, DH);
+            constexpr uint32_t idesc_qk = ns_idesc(1, 1, 0, 0, 128, ST_KB / L::KEYS), idesc_pv = ns_idesc(1, 1, 0, 1, 128, DH);
             const uint64_t desc_k = ns_desc_base(16, 1024);
             const uint64_t desc_v = ns_desc_base(L::HALF, 1024);      // MN-major: the halves of 64 columns, 8 key rows 1 KB apart
             Ring<L::SLOTS> kr, vr;
@@ -340,9 +349,11 @@ __global__ void __launch_bounds__(ST_THREADS, 1) ns_attention_shared_tile_kernel
                 if (leader) {
                     const uint32_t kb = smem_base + L::K_AT + kr.s * L::KV, qb = smem_base + L::Q * g, s_tmem = tmem_base + 256 * g + ST_S_COL;
 #pragma unroll
-                    for (int kk = 0; kk < DH / 16; kk++)
-                        ns_mma_f16(s_tmem, ns_desc_at(desc_k, qb + (kk >> 2) * (128 * 128) + (kk & 3) * 32),
-                                   ns_desc_at(desc_k, kb + (kk >> 2) * L::HALF + (kk & 3) * 32), idesc_qk, kk > 0 ? 1u : 0u);
+                    for (int e = 0; e < L::KEYS; e++)
+#pragma unroll
+                        for (int kk = 0; kk < DH / 16; kk++)
+                            ns_mma_f16(s_tmem + e * 64, ns_desc_at(desc_k, qb + (kk >> 2) * (128 * 128) + (kk & 3) * 32),
+                                       ns_desc_at(desc_k, kb + (kk >> 2) * L::HALF + (kk & 3) * 32 + e * 64), idesc_qk, kk > 0 ? 1u : 0u);
                     ns_tc_commit(bar(L::S_FULL + g));
                     if (free) ns_tc_commit(bar(L::K_EMPTY + kr.s));
                 }
@@ -369,7 +380,7 @@ __global__ void __launch_bounds__(ST_THREADS, 1) ns_attention_shared_tile_kernel
                             if (!ok) break;
                             ns_tc_fence_after();
                             if (leader) {
-                                const uint32_t vb = smem_base + L::V_AT + vr.s * L::KV + hf * (64 * 128), pa = s_tmem + hf * 32;
+                                const uint32_t vb = smem_base + L::V_AT + vr.s * L::KV + hf * (L::TWO ? 64 : 64 * 128), pa = s_tmem + hf * 32;
 #pragma unroll
                                 for (int kk = 0; kk < 4; kk++)
                                     st_mma_ts(o_tmem, pa + kk * 8, ns_desc_at(desc_v, vb + kk * (16 * 128)), idesc_pv, j - t.b0 >= step || hf > 0 || kk > 0 ? 1u : 0u);
@@ -430,21 +441,21 @@ __global__ void __launch_bounds__(ST_THREADS, 1) ns_attention_shared_tile_kernel
             // the warp's 32 queries, whole rows side by side: 16-byte piece c of row r at c ^ (r & 7).  (The group's scores before have all been computed: each warp
             // has waited for the last.)
             {
-                constexpr int CH = DH / 8, PER = 32 / CH;             // pieces of a row, rows at a time
+                constexpr int CH = DH / 8, PER = 32 / CH, UQ = 32 / PER < 8 ? 32 / PER : 8;      // pieces of a row, rows at a time, of those on their way
                 const int c = lane % CH, r0 = quad * 32 + lane / CH, base = row - r;
                 // (few instructions: this code is fetched cold, and unrolled with its divisions it took 7 000 cycles)
                 const int64_t head = (int64_t)t.kvh * p.s.group * DH + c * 8;
 #pragma unroll 1
-                for (int i = 0; i < 32; i += 8 * PER) {
-                    uint4 w[8];
+                for (int i = 0; i < 32; i += UQ * PER) {
+                    uint4 w[UQ];
 #pragma unroll
-                    for (int u = 0; u < 8; u++) {
+                    for (int u = 0; u < UQ; u++) {
                         const int rr = base + r0 + i + u * PER, token = p.group.of(rr);
                         w[u] = make_uint4(0, 0, 0, 0);
                         if (rr < p.rows) w[u] = *reinterpret_cast<const uint4*>(p.s.q + head + (int64_t)token * p.s.q_stride + (rr - token * p.s.group) * DH);
                     }
 #pragma unroll
-                    for (int u = 0; u < 8; u++) {
+                    for (int u = 0; u < UQ; u++) {
                         const int rr = r0 + i + u * PER;
                         ns_st_shared_v4(q_smem + (c >> 3) * (128 * 128) + rr * 128 + (((c & 7) ^ (rr & 7)) * 16), w[u].x, w[u].y, w[u].z, w[u].w);
                     }
@@ -478,14 +489,14 @@ __global__ void __launch_bounds__(ST_THREADS, 1) ns_attention_shared_tile_kernel
                 if (__builtin_expect(live < ST_KB, 0)) {
 #pragma unroll
                     for (int c = 0; c < ST_KB; c++)
-                        if (c >= live) s[c] = -INFINITY;
+                        if (L::key(c) >= live) s[c] = -INFINITY;
                 }
                 if (__builtin_expect(any_bad, 0)) {
                     const uint32_t bad = __ballot_sync(0xffffffffu, box_bad(j, box_page(j)));
                     const int box_shift = 31 - __clz(p.box);
 #pragma unroll
                     for (int c = 0; c < ST_KB; c++)
-                        if ((bad >> (c >> box_shift)) & 1u) s[c] = -INFINITY;
+                        if ((bad >> (L::key(c) >> box_shift)) & 1u) s[c] = -INFINITY;
                 }
                 // The reference maximum is raised only when the row maximum outgrew it by more than 8 in units of the exponent -- and in the first 512 keys
                 // whenever it grew: the largest weight is then exactly 1, which counts where a row has few keys.
@@ -606,9 +617,9 @@ int launch_tiles(NsDevice* d, const TileParams& p)
     using L = Layout<DH>;
     TileMaps maps;
     const int page = 1 << p.s.page_shift;
-    uint64_t dims[4] = {(uint64_t)DH, (uint64_t)page, (uint64_t)p.s.kv_heads, (uint64_t)p.s.num_pages};
-    uint64_t bytes[3] = {(uint64_t)DH * 2, (uint64_t)page * DH * 2, (uint64_t)p.s.kv_heads * page * DH * 2};
-    uint32_t box[4] = {64, (uint32_t)p.box, 1, 1};
+    uint64_t dims[4] = {(uint64_t)DH * L::KEYS, (uint64_t)page / L::KEYS, (uint64_t)p.s.kv_heads, (uint64_t)p.s.num_pages};
+    uint64_t bytes[3] = {(uint64_t)DH * 2 * L::KEYS, (uint64_t)page * DH * 2, (uint64_t)p.s.kv_heads * page * DH * 2};
+    uint32_t box[4] = {64, (uint32_t)(p.box / L::KEYS), 1, 1};
     int rc = ns_make_tensor_map(&maps.k, CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, 4, p.s.k_pool, dims, bytes, box, CU_TENSOR_MAP_SWIZZLE_128B);
     if (rc == NS_OK) rc = ns_make_tensor_map(&maps.v, CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, 4, p.s.v_pool, dims, bytes, box, CU_TENSOR_MAP_SWIZZLE_128B);
     if (rc != NS_OK) return rc;
@@ -630,7 +641,7 @@ bool ns_attention_shared_tiles_fit(const NsDevice* d, const SharedParams& s, int
 {
     // boxes of fewer than 8 rows would not begin on the swizzle's 1 KB; the reference maximum is one of raw scores, so their order has to be that of
     // the scaled ones
-    if (head_dim < 64 || s.page_shift < 3 || !(scale > 0.0f) || s.prefix_pages == 0) return false;
+    if (s.page_shift < (head_dim == 32 ? 4 : 3) || !(scale > 0.0f) || s.prefix_pages == 0) return false;
     // Little to multiply is the walking kernel's, which starts at once; so is what few rows have to read of long keys, which it has on their way from more places.  Both sides of the
     // line, us, this kernel's way and the other's (rows of a key/value head x heads x keys x columns): 32 x 8 x 2000 x 128 15.2, 16.0; 64 x 2 x 8000 x 128 19.5, 21.2; 128 x 8 x 2000 x 128 20.7,
     // 28.6; 64 x 8 x 2000 x 64 14.2, 14.9; 64 x 1 x 8000 x 128 15.9, 15.7; 256 x 2 x 2000 x 64 16.9, 14.9; 8 x 8 x 8000 x 128 23.7, 15.8; 16 x 16 x 8000 x 128 32.6, 30.2.
@@ -646,5 +657,5 @@ int ns_attention_shared_tiles(NsDevice* d, const SharedParams& s, int head_dim)
 {
     TileParams p;
     tile_plan(d, s, p);
-    return head_dim == 64 ? launch_tiles<64>(d, p) : launch_tiles<128>(d, p);
+    return head_dim == 32 ? launch_tiles<32>(d, p) : head_dim == 64 ? launch_tiles<64>(d, p) : launch_tiles<128>(d, p);
 }
