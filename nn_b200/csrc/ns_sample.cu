@@ -6,8 +6,8 @@
 // weights add up to p times all of theirs; of those the ones with w >= min_p.  The drawn token is the first in the order of the vocabulary at which the
 // running sum of kept weights exceeds u times their sum.
 //
-// A draw is decided by whether a sum of up to 10^5 weights lies left or right of a border, so the weights are computed in 64 bits and summed as integers
-// of 2^-42: exact, whatever the order, the number of CTAs or the atomics.  (With 32-bit weights one row in a few thousand draws another token than the
+// A draw is decided by whether a sum of up to 10^5 weights lies left or right of a border, so the weights are computed to 2^-33 of themselves and summed as
+// integers of 2^-42: exact, whatever the order, the number of CTAs or the atomics.  (With 32-bit weights one row in a few thousand draws another token than the
 // definition's.)
 //
 // A cluster of 1 to 8 CTAs holds a row in shared memory; it is read from global memory once.  What remains costs passes over shared memory:
@@ -93,10 +93,7 @@ struct alignas(16) SampleShared {
     uint64_t part[ST_MAX_CLUSTER], draw[ST_MAX_CLUSTER];       // of every CTA of the cluster, written between its barriers
     uint64_t extra[ST_THREADS];            // of each thread's run
     uint64_t scan[ST_THREADS / 32], scan2[ST_THREADS / 32];
-    float max[ST_MAX_CLUSTER];
-    int max_at[ST_MAX_CLUSTER];
-    float red[ST_THREADS / 32];
-    int red_at[ST_THREADS / 32];
+    float max[ST_MAX_CLUSTER], red[ST_THREADS / 32];
     SampleFound found;
     uint64_t cut;
     int run_first, run_end;
@@ -105,9 +102,39 @@ struct alignas(16) SampleShared {
 
 __device__ __forceinline__ float st_value(float x) { return x; }
 __device__ __forceinline__ float st_value(uint16_t x) { return ns_bf16_bits_to_f32(x); }
-// as a token is kept: what is no number counts as -infinity, and both zeros are one value
-__device__ __forceinline__ float st_clean(float x) { return x != x ? -INFINITY : x + 0.0f; }
-__device__ __forceinline__ uint16_t st_clean(uint16_t x) { return (x & 0x7FFF) > 0x7F80 ? 0xFF80 : x == 0x8000 ? 0 : x; }
+// As a token is kept: what is no number counts as -infinity (a maximum leaves NaN out), and both zeros are one value (adding 0 gives the positive one).
+__device__ __forceinline__ float st_clean(float x) { return fmaxf(x + 0.0f, -INFINITY); }
+__device__ __forceinline__ uint32_t st_clean2(uint32_t x)
+{
+    uint32_t y;
+    asm("{\n\t.reg .b32 t;\n\tadd.bf16x2 t, %1, %2;\n\tmax.bf16x2 %0, t, %3;\n\t}" : "=r"(y) : "r"(x), "r"(0u), "r"(0xFF80FF80u));
+    return y;
+}
+__device__ __forceinline__ uint16_t st_clean(uint16_t x) { return (uint16_t)st_clean2(x); }
+__device__ __forceinline__ uint32_t st_max2(uint32_t a, uint32_t b)
+{
+    uint32_t y;
+    asm("max.bf16x2 %0, %1, %2;" : "=r"(y) : "r"(a), "r"(b));
+    return y;
+}
+// a vector of tokens as they are kept; best: the largest so far
+__device__ __forceinline__ void st_take(uint4& v, float& best, const float*)
+{
+    float* e = reinterpret_cast<float*>(&v);
+#pragma unroll
+    for (int i = 0; i < 4; i++) {
+        e[i] = st_clean(e[i]);
+        best = fmaxf(best, e[i]);
+    }
+}
+__device__ __forceinline__ void st_take(uint4& v, float& best, const uint16_t*)
+{
+    uint32_t* e = reinterpret_cast<uint32_t*>(&v);
+#pragma unroll
+    for (int i = 0; i < 4; i++) e[i] = st_clean2(e[i]);
+    const uint32_t m = st_max2(st_max2(e[0], e[1]), st_max2(e[2], e[3]));
+    best = fmaxf(best, fmaxf(__uint_as_float(m << 16), __uint_as_float(m & 0xFFFF0000u)));
+}
 // ascending where the value descends
 __device__ __forceinline__ uint32_t st_key(float x)
 {
@@ -130,10 +157,38 @@ __device__ __forceinline__ uint64_t st_aim(float u, uint64_t total)
     return aim >= total ? total - 1 : aim;
 }
 
-// e^(-d / T) in units of 2^-42, d = max - x >= 0, within 2^-34 of itself (64-bit floats would take five times as long here: a warp's instruction 16 cycles).
+// e^(-d / T) in units of 2^-42, d = max - x >= 0, within 2^-33 of itself (64-bit floats would take five times as long here: a warp's instruction 16 cycles).
 // d is a float and the rest of it, exactly; t = d / (T ln 2) the same to 2^-46 of itself; t = n + i / 1024 + r with |r| <= 2^-11;
 // 2^(-i / 1024) from a table, 2^(-r) = 1 + q with q a polynomial of degree 3 and below 2^-12, so that its float's error counts 2^-36; the product is rounded to an
 // integer once, and shifted by n.
+__device__ __forceinline__ uint64_t st_pair(float lo, float hi)
+{
+    uint64_t y;
+    asm("mov.b64 %0, {%1, %2};" : "=l"(y) : "f"(lo), "f"(hi));
+    return y;
+}
+__device__ __forceinline__ void st_split(uint64_t v, float& lo, float& hi) { asm("mov.b64 {%0, %1}, %2;" : "=f"(lo), "=f"(hi) : "l"(v)); }
+// two sums, products, fused multiply-adds: each rounded as the single ones are
+__device__ __forceinline__ uint64_t st_add2(uint64_t a, uint64_t b)
+{
+    uint64_t y;
+    asm("add.rn.f32x2 %0, %1, %2;" : "=l"(y) : "l"(a), "l"(b));
+    return y;
+}
+__device__ __forceinline__ uint64_t st_mul2(uint64_t a, uint64_t b)
+{
+    uint64_t y;
+    asm("mul.rn.f32x2 %0, %1, %2;" : "=l"(y) : "l"(a), "l"(b));
+    return y;
+}
+__device__ __forceinline__ uint64_t st_fma2(uint64_t a, uint64_t b, uint64_t c)
+{
+    uint64_t y;
+    asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(y) : "l"(a), "l"(b), "l"(c));
+    return y;
+}
+__device__ __forceinline__ uint64_t st_neg2(uint64_t a) { return a ^ 0x8000000080000000ull; }
+
 struct SampleWeight {
     float max, rate, rate_lo;              // 1 / (T ln 2): the float and the rest of it
     const SampleTable* table;
@@ -143,24 +198,41 @@ struct SampleWeight {
         rate = (float)fmin(r, 3e38);
         rate_lo = (float)(fmin(r, 3e38) - (double)rate);
     }
+    // of p, its steps of 1/1024 as the bits of ni, and 2^-r - 1
+    __device__ __forceinline__ uint64_t finish(float x, float p, float ni, float q) const
+    {
+        const int steps = __float_as_int(ni) - 0x4B400000, i = steps & (ST_TABLE - 1), n = (steps >> 10) & 63;        // n * 1024 + i
+        const uint64_t w = table->fixed[i] + (int64_t)__float2int_rn(table->value[i] * q);
+        const uint64_t rounded = (w + (1ull << n >> 1)) >> n;
+        // both ends: equal to the maximum (infinities among them), and too far for half a unit
+        return x == max ? 1ull << ST_FIX : p < (float)(ST_FIX + 2) ? rounded : 0;
+    }
+    // The weights of two tokens.
+    __device__ __forceinline__ void two(float x0, float x1, uint64_t& w0, uint64_t& w1) const
+    {
+        const uint64_t x = st_pair(x0, x1), m = st_pair(max, max), r2 = st_pair(rate, rate), magic = st_pair(12582912.0f, 12582912.0f);       // 1.5 * 2^23: a sum's low bits are the rounded value
+        const uint64_t d = st_add2(m, st_neg2(x)), p = st_mul2(d, r2);
+        float p0, p1;
+        st_split(p, p0, p1);
+        w0 = w1 = 0;
+        if (!(fminf(p0, p1) < (float)(ST_FIX + 2)) && x0 != max && x1 != max) return;
+        // d + d_lo = max - x
+        const uint64_t back = st_add2(d, st_neg2(m)), d_lo = st_add2(st_add2(m, st_neg2(st_add2(d, st_neg2(back)))), st_neg2(st_add2(x, back)));
+        const uint64_t p_lo = st_fma2(d_lo, r2, st_fma2(d, st_pair(rate_lo, rate_lo), st_fma2(d, r2, st_neg2(p))));
+        const uint64_t ni = st_fma2(p, st_pair(1024.0f, 1024.0f), magic);
+        const uint64_t r = st_add2(st_fma2(st_add2(ni, st_neg2(magic)), st_pair(-0.0009765625f, -0.0009765625f), p), p_lo);      // (the product and its sum are exact)
+        const uint64_t q = st_mul2(r, st_fma2(r, st_fma2(r, st_pair(-0.055504109f, -0.055504109f), st_pair(0.24022651f, 0.24022651f)), st_pair(-0.69314718f, -0.69314718f)));
+        float n0, n1, q0, q1;
+        st_split(ni, n0, n1);
+        st_split(q, q0, q1);
+        w0 = finish(x0, p0, n0, q0);
+        w1 = finish(x1, p1, n1, q1);
+    }
     __device__ __forceinline__ uint64_t operator()(float x) const
     {
-        // both ends first: equal (infinities among them), and too far for half a unit
-        if (x == max) return 1ull << ST_FIX;
-        const float d = __fsub_rn(max, x);
-        const float p = __fmul_rn(d, rate);
-        if (!(p < (float)(ST_FIX + 2))) return 0;
-        // d + d_lo = max - x
-        const float back = __fsub_rn(d, max), d_lo = __fsub_rn(__fsub_rn(max, __fsub_rn(d, back)), __fadd_rn(x, back));
-        const float p_lo = fmaf(d_lo, rate, fmaf(d, rate_lo, fmaf(d, rate, -p)));
-        const float magic = 12582912.0f;   // 1.5 * 2^23: a sum's low bits are the rounded value
-        const float ni = fmaf(p, 1024.0f, magic);
-        const int steps = __float_as_int(ni) - __float_as_int(magic);          // n * 1024 + i
-        const float r = __fadd_rn(fmaf(__fsub_rn(ni, magic), -0.0009765625f, p), p_lo);        // (the product and its sum are exact)
-        const float q = r * fmaf(r, fmaf(r, -0.055504109f, 0.24022651f), -0.69314718f);        // 2^-r - 1
-        const int i = steps & (ST_TABLE - 1), n = steps >> 10;
-        const uint64_t w = table->fixed[i] + (int64_t)__float2int_rn(table->value[i] * q);
-        return n == 0 ? w : (w + (1ull << (n - 1))) >> n;
+        uint64_t w0, w1;
+        two(x, -INFINITY, w0, w1);
+        return w0;
     }
 };
 
@@ -186,8 +258,6 @@ __device__ __forceinline__ uint64_t st_scan(uint64_t v, uint64_t* warps, uint64_
     }
     return before + inc - v;
 }
-
-__device__ __forceinline__ bool st_better(float v, int i, float w, int j) { return v > w || (v == w && i < j); }
 
 // the first histogram's bin: scale = 64 / T
 __device__ __forceinline__ int st_coarse(float x, float max, float scale)
@@ -275,6 +345,25 @@ struct SampleRow {
 #pragma unroll
                 for (int i = 0; i < VEC; i++)
                     if (i0 + i >= 0 && i0 + i < n) f(i0 + i, st_value(e[i]));
+            }
+        }
+    }
+    // f(number in the CTA of the first, value, value) for pairs of neighbouring tokens, -infinity where there is none
+    template <typename F>
+    __device__ __forceinline__ void pairs(int at, int step, int end, F f) const
+    {
+        const uint4* vecs = reinterpret_cast<const uint4*>(vals - skew);
+        for (int v = at; v < end; v += step) {
+            const uint4 raw = vecs[v];
+            const T* e = reinterpret_cast<const T*>(&raw);
+            const int i0 = v * VEC - skew;
+            if (i0 >= 0 && i0 + VEC <= n) {
+#pragma unroll
+                for (int i = 0; i < VEC; i += 2) f(i0 + i, st_value(e[i]), st_value(e[i + 1]));
+            } else {
+#pragma unroll
+                for (int i = 0; i < VEC; i += 2)
+                    f(i0 + i, i0 + i >= 0 && i0 + i < n ? st_value(e[i]) : -INFINITY, i0 + i + 1 >= 0 && i0 + i + 1 < n ? st_value(e[i + 1]) : -INFINITY);
             }
         }
     }
@@ -404,9 +493,18 @@ struct SampleRow {
     __device__ SampleCut select(bool mass, uint64_t limit, const SampleWeight& weight, uint64_t least, uint64_t& sum, G goal)
     {
         clear(mass);
-        all([&](int i, float x) {
-            if (limit == ~0ull || place(i, x) <= limit) put(mass, coarse(x), mass ? weight(x) : 0);
-        });
+        if (mass) {
+            pairs(threadIdx.x, ST_THREADS, vectors(), [&](int i, float x0, float x1) {
+                uint64_t w0, w1;
+                weight.two(x0, x1, w0, w1);
+                if (limit == ~0ull || place(i, x0) <= limit) put(true, coarse(x0), w0);
+                if (limit == ~0ull || place(i + 1, x1) <= limit) put(true, coarse(x1), w1);
+            });
+        } else {
+            all([&](int i, float x) {
+                if (limit == ~0ull || place(i, x) <= limit) put(false, coarse(x), 0);
+            });
+        }
         uint64_t target = 0;
         SampleFound f = find(mass, [&](uint64_t whole) {
             target = goal(whole);
@@ -491,15 +589,12 @@ __global__ void __launch_bounds__(ST_THREADS) ns_sample_tokens_kernel(const Samp
 #pragma unroll
     for (int i = 0; i < ST_TABLE / ST_THREADS; i++) power[i] = st_powers.v[tid + i * ST_THREADS];
     float best = -INFINITY;
-    int best_at = p.vocab;
-    auto take = [&](T raw, int i) {
-        const T kept = st_clean(raw);
-        const float v = st_value(kept);
-        if (v > best) { best = v; best_at = first + i; }
-        return kept;
-    };
     const int head = min(n, skew == 0 ? 0 : VEC - skew), vecs = (n - head) / VEC, tail = head + vecs * VEC;
-    if (tid < head) vals[tid] = take(src[tid], tid);
+    auto take_one = [&](int i) {
+        vals[i] = st_clean(src[i]);
+        best = fmaxf(best, st_value(vals[i]));
+    };
+    if (tid < head) take_one(tid);
     {
         constexpr int U = 4;
         const uint4* from = reinterpret_cast<const uint4*>(src + head);
@@ -512,53 +607,53 @@ __global__ void __launch_bounds__(ST_THREADS) ns_sample_tokens_kernel(const Samp
 #pragma unroll
             for (int u = 0; u < U; u++)
                 if (at + u * ST_THREADS < vecs) {
-                    T* e = reinterpret_cast<T*>(&v[u]);
-#pragma unroll
-                    for (int i = 0; i < VEC; i++) e[i] = take(e[i], head + (at + u * ST_THREADS) * VEC + i);
+                    st_take(v[u], best, src);
                     to[at + u * ST_THREADS] = v[u];
                 }
         }
     }
-    if (tail + tid < n) vals[tail + tid] = take(src[tail + tid], tail + tid);
-
+    if (tail + tid < n) take_one(tail + tid);
 #pragma unroll
     for (int i = 0; i < ST_TABLE / ST_THREADS; i++) {
         s.table.fixed[tid + i * ST_THREADS] = power[i];
         s.table.value[tid + i * ST_THREADS] = (float)power[i];
     }
-    // ---- the first maximum
+    // ---- the maximum
 #pragma unroll
-    for (int o = 16; o > 0; o >>= 1) {
-        const float v = __shfl_xor_sync(0xffffffffu, best, o);
-        const int i = __shfl_xor_sync(0xffffffffu, best_at, o);
-        if (st_better(v, i, best, best_at)) { best = v; best_at = i; }
-    }
-    if ((tid & 31) == 0) { s.red[tid >> 5] = best; s.red_at[tid >> 5] = best_at; }
+    for (int o = 16; o > 0; o >>= 1) best = fmaxf(best, __shfl_xor_sync(0xffffffffu, best, o));
+    if ((tid & 31) == 0) s.red[tid >> 5] = best;
     __syncthreads();
     if (tid < ranks) {
-        for (int w = 0; w < ST_THREADS / 32; w++)
-            if (w == 0 || st_better(s.red[w], s.red_at[w], best, best_at)) { best = s.red[w]; best_at = s.red_at[w]; }
-        SampleShared* o = cl.map_shared_rank(&s, tid);
-        o->max[rank] = best;
-        o->max_at[rank] = best_at;
+        for (int w = 0; w < ST_THREADS / 32; w++) best = fmaxf(best, s.red[w]);
+        cl.map_shared_rank(&s, tid)->max[rank] = best;
     }
     cl.sync();
     float max = s.max[0];
-    int max_at = s.max_at[0];
-    for (int r = 1; r < ranks; r++)
-        if (st_better(s.max[r], s.max_at[r], max, max_at)) { max = s.max[r]; max_at = s.max_at[r]; }
+    for (int r = 1; r < ranks; r++) max = fmaxf(max, s.max[r]);
 
     if (k <= 0 || k > p.vocab) k = p.vocab;
-    // greedily, or nothing to choose from: every CTA sees the same and leaves
+    SampleRow<T> me{s, vals, n, first, skew, cl, rank, ranks, max, fminf(64.0f / temperature, 1e30f)};
+    // Greedily, or nothing to choose from: every CTA sees the same and leaves, the first that has the maximum once it has found where.
     if (max == -INFINITY || !(temperature > 0.0f) || k == 1) {
-        if (rank == 0 && tid == 0) {
-            p.ids[row] = max == -INFINITY ? -1 : max_at;
-            if (p.probs != nullptr) p.probs[row] = max == -INFINITY ? 0.0f : 1.0f;
+        int owner = 0;
+        while (s.max[owner] != max) owner++;
+        if (rank == owner) {
+            if (tid == 0) s.mine = n;
+            __syncthreads();
+            int at = n;
+            me.all([&](int i, float x) {
+                if (x == max) at = min(at, i);
+            });
+            if (at < n) atomicMin(&s.mine, at);
+            __syncthreads();
+            if (tid == 0) {
+                p.ids[row] = max == -INFINITY ? -1 : first + s.mine;
+                if (p.probs != nullptr) p.probs[row] = max == -INFINITY ? 0.0f : 1.0f;
+            }
         }
         return;
     }
     const SampleWeight weight(max, temperature, &s.table);
-    SampleRow<T> me{s, vals, n, first, skew, cl, rank, ranks, max, fminf(64.0f / temperature, 1e30f)};
     uint64_t least = 0;
     if (min_p > 0.0f) least = (uint64_t)ceil((double)fminf(min_p, 1.0f) * (double)(1ull << ST_FIX));
 
@@ -576,7 +671,9 @@ __global__ void __launch_bounds__(ST_THREADS) ns_sample_tokens_kernel(const Samp
         for (int i = (every - first % every) % every + tid * every; i < n; i += ST_THREADS * every) me.put(false, me.coarse(st_value(vals[i])), 0);
         const int bin = me.find(false, [&](uint64_t sample) { return need < sample ? need : sample; }).bin;
         int count = 0;
-        count = me.gather([&](int, float x) { return me.coarse(x) <= bin; });
+        // (about the tokens of those bins: as many as k of them is what counts)
+        const float near = max - ((float)bin + 0.5f) * (temperature * (1.0f / 64));
+        count = me.gather([&](int, float x) { return x >= near; });
         if (count >= k) {
             cl.sync();                     // the first CTA has the others' lists
             if (rank != 0) return;
@@ -603,7 +700,15 @@ __global__ void __launch_bounds__(ST_THREADS) ns_sample_tokens_kernel(const Samp
     };
     if (cut.bin < 0) {
         sum = 0;
-        me.run([&](int i, float x) { sum += kept(i, x); });
+        if (cut.last == ~0ull) {
+            me.pairs(me.run_begin(tid), 1, me.run_begin(tid + 1), [&](int, float x0, float x1) {
+                uint64_t w0, w1;
+                weight.two(x0, x1, w0, w1);
+                sum += (w0 >= least ? w0 : 0) + (w1 >= least ? w1 : 0);
+            });
+        } else {
+            me.run([&](int i, float x) { sum += kept(i, x); });
+        }
     } else {
         // all but the cutoff's bin are in the sums: its tokens are this CTA's part of the lists
         s.extra[tid] = 0;
