@@ -11,10 +11,11 @@
 // definition's.)
 //
 // A cluster of 1 to 8 CTAs holds a row in shared memory; it is read from global memory once.  What remains costs passes over shared memory:
-//   - A top-k of up to ST_SORT_K: a histogram of every 16th token over (max - x) / T in steps of 1/64 names a cutoff that hardly ever fails to leave k candidates and leaves
+//   - A top-k of up to ST_SORT_K: a histogram of every 8th token over (max - x) / T, 45 bins to each halving of the weight, names a cutoff that hardly ever fails to leave k candidates and leaves
 //     few more; they are gathered into one CTA, sorted (value, then index), cut by all three rules, sorted by index and drawn from.
-//   - Else cutoffs are found one after the other: the histogram of all tokens, by number or by weight, names the bin in which a cutoff lies, and that bin's tokens alone
-//     are gathered and sorted (or, where they are too many, counted by the bits of x, 11 at a time).  The draw is then one more pass over the row.
+//   - Else cutoffs are found one after the other: a histogram, by number (from such a cutoff on) or by weight, names the bin in which a cutoff lies, and that bin's tokens
+//     alone are gathered and sorted (or, where they are too many, counted by the bits of x, 11 at a time).  The draw is then one more pass over the row, or, after a
+//     cutoff by weight, the sums of the pass that gathered.
 #include <cooperative_groups.h>
 #include <math.h>
 
@@ -28,11 +29,13 @@ constexpr int ST_THREADS = 512;
 constexpr int ST_BINS = 2048;
 constexpr int ST_MAX_CLUSTER = 8;
 constexpr int ST_FIX = 42;                 // weights are multiples of 2^-42: 2^20 of them fit 64 bits
+constexpr int ST_FAR = 45;                 // 2^-45 and less is no weight
+constexpr int ST_OCTAVE = 45;              // bins of the first histogram that halve the weight
+constexpr float ST_MAGIC = 12582912.0f;    // 1.5 * 2^23: the low bits of a sum with it are the rounded value
 constexpr int ST_TABLE = 1024;             // 2^(-i / 1024)
 constexpr int ST_LIST = ST_THREADS;         // candidates that are sorted: one a thread
 constexpr int ST_SORT_K = 128;             // the largest top-k whose candidates they are
-constexpr int ST_SAMPLE = 16;              // its cutoff is guessed from every 16th token
-constexpr int ST_LIMB = 14;                // bits of a weight's share of a histogram's word: 2^18 of them fit
+constexpr int ST_SAMPLE = 8;               // its cutoff is guessed from every 8th token
 constexpr uint32_t ST_NO_CUT = 0xFFFFFFFFu;
 
 struct SampleArgs {
@@ -49,8 +52,8 @@ struct SampleArgs {
 };
 
 struct SampleTable {
-    uint64_t fixed[ST_TABLE];              // in units of 2^-42
-    float value[ST_TABLE];                 // the same as floats, times 2^42
+    uint64_t twice[ST_TABLE];              // in units of 2^-43
+    float value[ST_TABLE];                 // in units of 2^-42
 };
 
 // 2^42 * 2^(-i / 1024), rounded, made by the compiler from the series of e^x (64-bit exponentials would take every CTA microseconds).
@@ -81,11 +84,12 @@ struct SampleCut {
 struct alignas(16) SampleShared {
     union {
         struct {
-            uint32_t word[3][ST_BINS];     // numbers, or weights in three shares of ST_LIMB bits
+            uint32_t word[2][ST_BINS];     // numbers, or weights: the low word, the high word
         };
         struct {
             __align__(16) uint64_t list[ST_LIST];        // candidates: key, index
             uint64_t sorted[ST_LIST], weights[ST_LIST];
+            int ranks[ST_THREADS];
         };
     };
     int listed[ST_MAX_CLUSTER], mine;
@@ -101,6 +105,8 @@ struct alignas(16) SampleShared {
 };
 
 __device__ __forceinline__ float st_value(float x) { return x; }
+__device__ __forceinline__ float st_bits(float x, const float*) { return x; }
+__device__ __forceinline__ uint16_t st_bits(float x, const uint16_t*) { return (uint16_t)(__float_as_uint(x) >> 16); }       // (of zero and infinity)
 __device__ __forceinline__ float st_value(uint16_t x) { return ns_bf16_bits_to_f32(x); }
 // As a token is kept: what is no number counts as -infinity (a maximum leaves NaN out), and both zeros are one value (adding 0 gives the positive one).
 __device__ __forceinline__ float st_clean(float x) { return fmaxf(x + 0.0f, -INFINITY); }
@@ -135,6 +141,52 @@ __device__ __forceinline__ void st_take(uint4& v, float& best, const uint16_t*)
     const uint32_t m = st_max2(st_max2(e[0], e[1]), st_max2(e[2], e[3]));
     best = fmaxf(best, fmaxf(__uint_as_float(m << 16), __uint_as_float(m & 0xFFFF0000u)));
 }
+// what is below `value` becomes -infinity; ties: something equals it
+__device__ __forceinline__ void st_erase(uint4& v, float value, bool& ties, const float*)
+{
+    float* e = reinterpret_cast<float*>(&v);
+#pragma unroll
+    for (int i = 0; i < 4; i++) {
+        ties = ties || e[i] == value;
+        e[i] = e[i] < value ? -INFINITY : e[i];
+    }
+}
+__device__ __forceinline__ void st_erase(uint4& v, float value, bool& ties, const uint16_t*)
+{
+    uint32_t* e = reinterpret_cast<uint32_t*>(&v);
+    const uint32_t both = __byte_perm(__float_as_uint(value), 0, 0x3232);
+    uint32_t equal = 0;
+#pragma unroll
+    for (int i = 0; i < 4; i++) {
+        uint32_t less, same;
+        asm("set.lt.u32.bf16x2 %0, %1, %2;" : "=r"(less) : "r"(e[i]), "r"(both));
+        asm("set.eq.u32.bf16x2 %0, %1, %2;" : "=r"(same) : "r"(e[i]), "r"(both));
+        equal |= same;
+        e[i] = (e[i] & ~less) | (0xFF80FF80u & less);
+    }
+    ties = equal != 0;
+}
+// Which of a vector's tokens reach `floor` (a bf16): of 4, a bit each; of 8, the even ones in the low half and the odd ones in the high half, two bits each.
+__device__ __forceinline__ uint32_t st_reach(const uint4& v, float floor, const float*)
+{
+    const float* e = reinterpret_cast<const float*>(&v);
+    return (e[0] >= floor ? 1 : 0) | (e[1] >= floor ? 2 : 0) | (e[2] >= floor ? 4 : 0) | (e[3] >= floor ? 8 : 0);
+}
+__device__ __forceinline__ uint32_t st_reach(const uint4& v, float floor, const uint16_t*)
+{
+    const uint32_t* e = reinterpret_cast<const uint32_t*>(&v);
+    const uint32_t both = __byte_perm(__float_as_uint(floor), 0, 0x3232);
+    uint32_t mask = 0;
+#pragma unroll
+    for (int i = 0; i < 4; i++) {
+        uint32_t m;
+        asm("set.ge.u32.bf16x2 %0, %1, %2;" : "=r"(m) : "r"(e[i]), "r"(both));
+        mask |= m & (0x00010001u << (2 * i));
+    }
+    return mask;
+}
+__device__ __forceinline__ int st_reached(int bit, const float*) { return bit; }
+__device__ __forceinline__ int st_reached(int bit, const uint16_t*) { return (bit & 15) + (bit >> 4); }
 // ascending where the value descends
 __device__ __forceinline__ uint32_t st_key(float x)
 {
@@ -189,6 +241,14 @@ __device__ __forceinline__ uint64_t st_fma2(uint64_t a, uint64_t b, uint64_t c)
 }
 __device__ __forceinline__ uint64_t st_neg2(uint64_t a) { return a ^ 0x8000000080000000ull; }
 
+// a * b + c
+__device__ __forceinline__ uint64_t st_mad(int a, int b, uint64_t c)
+{
+    uint64_t y;
+    asm("mad.wide.s32 %0, %1, %2, %3;" : "=l"(y) : "r"(a), "r"(b), "l"(c));
+    return y;
+}
+
 struct SampleWeight {
     float max, rate, rate_lo;              // 1 / (T ln 2): the float and the rest of it
     const SampleTable* table;
@@ -198,36 +258,49 @@ struct SampleWeight {
         rate = (float)fmin(r, 3e38);
         rate_lo = (float)(fmin(r, 3e38) - (double)rate);
     }
-    // of p, its steps of 1/1024 as the bits of ni, and 2^-r - 1
-    __device__ __forceinline__ uint64_t finish(float x, float p, float ni, float q) const
+    // 2^-p in units of 2^-42, for p's steps of 1/1024 as the low bits of ni and q = 2^-rest - 1: the products add in 64 bits on the multipliers' pipe, the others are
+    // this kernel's bound
+    __device__ __forceinline__ uint64_t finish(float ni, float q) const
     {
-        const int steps = __float_as_int(ni) - 0x4B400000, i = steps & (ST_TABLE - 1), n = (steps >> 10) & 63;        // n * 1024 + i
-        const uint64_t w = table->fixed[i] + (int64_t)__float2int_rn(table->value[i] * q);
-        const uint64_t rounded = (w + (1ull << n >> 1)) >> n;
-        // both ends: equal to the maximum (infinities among them), and too far for half a unit
-        return x == max ? 1ull << ST_FIX : p < (float)(ST_FIX + 2) ? rounded : 0;
+        const int steps = __float_as_int(ni), i = steps & (ST_TABLE - 1), n = (steps >> 10) & 63;       // n * 1024 + i
+        const uint64_t w = st_mad(__float2int_rn(table->value[i] * q), 2, table->twice[i]);
+        return st_mad(1, 1, w >> n) >> 1;
     }
-    // The weights of two tokens.
-    __device__ __forceinline__ void two(float x0, float x1, uint64_t& w0, uint64_t& w1) const
+    // steps of 2^-1/1024 from the maximum down, as the low bits of ni: no more than for the largest p that leaves no weight (infinity and 0 * infinity become that too)
+    __device__ __forceinline__ float limit(float p) const { return fminf(p, (float)ST_FAR); }
+    // The weights of two tokens, and their bins.
+    __device__ __forceinline__ void two(float x0, float x1, uint64_t& w0, uint64_t& w1, int& b0, int& b1) const
     {
-        const uint64_t x = st_pair(x0, x1), m = st_pair(max, max), r2 = st_pair(rate, rate), magic = st_pair(12582912.0f, 12582912.0f);       // 1.5 * 2^23: a sum's low bits are the rounded value
-        const uint64_t d = st_add2(m, st_neg2(x)), p = st_mul2(d, r2);
+        const uint64_t x = st_pair(x0, x1), m = st_pair(max, max), r2 = st_pair(rate, rate), magic = st_pair(ST_MAGIC, ST_MAGIC);
+        const uint64_t d = st_add2(m, st_neg2(x));
         float p0, p1;
-        st_split(p, p0, p1);
+        st_split(st_mul2(d, r2), p0, p1);
+        const uint64_t p = st_pair(limit(p0), limit(p1));
+        const uint64_t ni = st_fma2(p, st_pair(1024.0f, 1024.0f), magic);
+        float n0, n1;
+        st_split(ni, n0, n1);
+        b0 = bin(n0);
+        b1 = bin(n1);
         w0 = w1 = 0;
-        if (!(fminf(p0, p1) < (float)(ST_FIX + 2)) && x0 != max && x1 != max) return;
+        if (fminf(p0, p1) >= (float)ST_FAR) return;
         // d + d_lo = max - x
         const uint64_t back = st_add2(d, st_neg2(m)), d_lo = st_add2(st_add2(m, st_neg2(st_add2(d, st_neg2(back)))), st_neg2(st_add2(x, back)));
         const uint64_t p_lo = st_fma2(d_lo, r2, st_fma2(d, st_pair(rate_lo, rate_lo), st_fma2(d, r2, st_neg2(p))));
-        const uint64_t ni = st_fma2(p, st_pair(1024.0f, 1024.0f), magic);
         const uint64_t r = st_add2(st_fma2(st_add2(ni, st_neg2(magic)), st_pair(-0.0009765625f, -0.0009765625f), p), p_lo);      // (the product and its sum are exact)
         const uint64_t q = st_mul2(r, st_fma2(r, st_fma2(r, st_pair(-0.055504109f, -0.055504109f), st_pair(0.24022651f, 0.24022651f)), st_pair(-0.69314718f, -0.69314718f)));
-        float n0, n1, q0, q1;
-        st_split(ni, n0, n1);
+        float q0, q1;
         st_split(q, q0, q1);
-        w0 = finish(x0, p0, n0, q0);
-        w1 = finish(x1, p1, n1, q1);
+        w0 = finish(n0, q0);           // (where p was limited, whatever q is leaves less than half a unit: the conversion saturates)
+        w1 = finish(n1, q1);
     }
+    __device__ __forceinline__ void two(float x0, float x1, uint64_t& w0, uint64_t& w1) const
+    {
+        int b0, b1;
+        two(x0, x1, w0, w1, b0, b1);
+    }
+    // The first histogram's bin, never less for a smaller token: ST_OCTAVE of them halve the weight.
+    __device__ __forceinline__ int bin(float ni) const { return (__float_as_int(ni) - 0x4B400000) * ST_OCTAVE >> 10; }
+    __device__ __forceinline__ int coarse(float x) const { return bin(fmaf(limit((max - x) * rate), 1024.0f, ST_MAGIC)); }
     __device__ __forceinline__ uint64_t operator()(float x) const
     {
         uint64_t w0, w1;
@@ -259,25 +332,28 @@ __device__ __forceinline__ uint64_t st_scan(uint64_t v, uint64_t* warps, uint64_
     return before + inc - v;
 }
 
-// the first histogram's bin: scale = 64 / T
-__device__ __forceinline__ int st_coarse(float x, float max, float scale)
+// Puts `count` different values of `from` into `to` in order.  Every value is compared with all others, by as many threads as there are for each.
+__device__ void st_sort(const uint64_t* from, uint64_t* to, int* ranks, int count)
 {
-    const float d = x == max ? 0.0f : max - x;
-    return __float_as_int(fminf(d * scale, (float)(ST_BINS - 1)) + 12582912.0f) - 0x4B400000;       // rounded by the sum with 1.5 * 2^23
-}
-
-// How many of `list`'s `count` values are below v (all different): every thread compares its own with all of them.
-__device__ __forceinline__ int st_rank(const uint64_t* list, int count, uint64_t v)
-{
-    int r = 0;
-    const ulonglong2* pairs = reinterpret_cast<const ulonglong2*>(list);
+    const int tid = threadIdx.x, shares = count <= ST_THREADS / 4 ? 4 : count <= ST_THREADS / 2 ? 2 : 1, width = ST_THREADS / shares;
+    const int i = tid & (width - 1), share = tid / width, per = ((count + shares - 1) / shares + 1) & ~1, first = min(share * per, count), end = min(first + per, count);
+    ranks[tid] = 0;
+    __syncthreads();
+    const uint64_t v = i < count ? from[i] : 0;
+    if (i < count) {
+        int r = 0, j = first;
+        const ulonglong2* pairs = reinterpret_cast<const ulonglong2*>(from);
 #pragma unroll 4
-    for (int j = 0; j < count / 2; j++) {
-        const ulonglong2 w = pairs[j];
-        r += (w.x < v ? 1 : 0) + (w.y < v ? 1 : 0);
+        for (; j + 1 < end; j += 2) {
+            const ulonglong2 w = pairs[j >> 1];
+            r += (w.x < v ? 1 : 0) + (w.y < v ? 1 : 0);
+        }
+        if (j < end) r += from[j] < v ? 1 : 0;
+        if (r != 0) atomicAdd(&ranks[i], r);
     }
-    if ((count & 1) != 0) r += list[count - 1] < v ? 1 : 0;
-    return r;
+    __syncthreads();
+    if (tid < count) to[ranks[tid]] = v;
+    __syncthreads();
 }
 
 struct SampleCuts {
@@ -290,11 +366,7 @@ struct SampleCuts {
 __device__ void st_draw(SampleShared& s, int count, const SampleCuts& cuts, const SampleWeight& weight, int row, const SampleArgs& p)
 {
     const int tid = threadIdx.x;
-    if (tid < count) {
-        const uint64_t v = s.list[tid];
-        s.sorted[st_rank(s.list, count, v)] = v;
-    }
-    __syncthreads();
+    st_sort(s.list, s.sorted, s.ranks, count);
     const uint64_t v = tid < count ? s.sorted[tid] : 0;
     uint64_t w = tid < count && tid < cuts.k ? weight(st_unkey((uint32_t)(v >> 32))) : 0, total;
     uint64_t before = st_scan(w, s.scan, total);
@@ -302,19 +374,14 @@ __device__ void st_draw(SampleShared& s, int count, const SampleCuts& cuts, cons
     // kept is the beginning; then by index
     const int kept = __syncthreads_count(tid < count && tid < cuts.k && before < goal && w >= cuts.least);
     if (tid < kept) s.list[tid] = v << 32 | (uint32_t)tid;
+    s.weights[tid] = w;
     __syncthreads();
-    if (tid < kept) {
-        const uint64_t mine = v << 32 | (uint32_t)tid;
-        const int at = st_rank(s.list, kept, mine);
-        s.sorted[at] = mine >> 32;
-        s.weights[at] = w;
-    }
-    __syncthreads();
-    w = tid < kept ? s.weights[tid] : 0;
+    st_sort(s.list, s.sorted, s.ranks, kept);
+    w = tid < kept ? s.weights[(uint32_t)s.sorted[tid]] : 0;
     before = st_scan(w, s.scan2, total);
     const uint64_t aim = st_aim(cuts.u, total);
     if (before <= aim && aim < before + w) {
-        p.ids[row] = (int)s.sorted[tid];
+        p.ids[row] = (int)(s.sorted[tid] >> 32);
         if (p.probs != nullptr) p.probs[row] = (float)((double)w / (double)total);
     }
 }
@@ -323,11 +390,11 @@ template <typename T>
 struct SampleRow {
     static constexpr int VEC = 16 / sizeof(T);
     SampleShared& s;
-    const T* vals;                         // this CTA's tokens; they begin `skew` after a vector
+    T* vals;                               // this CTA's tokens; they begin `skew` after a vector
     int n, first, skew;                    // how many, the first's index
     cg::cluster_group cl;
     int rank, ranks;
-    float max, scale;
+    const SampleWeight& weight;
 
     // f(number in the CTA, value) for its tokens: vectors first, first + step .. below end
     template <typename F>
@@ -367,6 +434,17 @@ struct SampleRow {
             }
         }
     }
+    // f(number in the CTA, value) for the tokens that reach `floor`, where they are few
+    template <typename F>
+    __device__ __forceinline__ void above(int at, int step, int end, float floor, F f) const
+    {
+        const uint4* vecs = reinterpret_cast<const uint4*>(vals - skew);
+        for (int v = at; v < end; v += step)
+            for (uint32_t mask = st_reach(vecs[v], floor, vals); mask != 0; mask &= mask - 1) {
+                const int i = v * VEC - skew + st_reached(__ffs((int)mask) - 1, vals);
+                if (i >= 0 && i < n) f(i, st_value(vals[i]));
+            }
+    }
     __device__ __forceinline__ int vectors() const { return n > 0 ? (n + skew + VEC - 1) / VEC : 0; }
     // a thread's run of neighbouring vectors: an odd number, so that neighbouring threads read from different banks
     __device__ __forceinline__ int run_length() const { return (vectors() + ST_THREADS - 1) / ST_THREADS | 1; }
@@ -376,12 +454,11 @@ struct SampleRow {
     __device__ __forceinline__ uint64_t place(int i, float x) const { return ((uint64_t)st_key(x) << 32) | (uint32_t)(first + i); }
     template <typename F>
     __device__ __forceinline__ void all(F f) const { each(threadIdx.x, ST_THREADS, vectors(), f); }
-    __device__ __forceinline__ int coarse(float x) const { return st_coarse(x, max, scale); }
 
     __device__ void clear(bool mass)
     {
         uint32_t* w = s.word[0];
-        for (int i = threadIdx.x; i < (mass ? 3 : 1) * ST_BINS; i += ST_THREADS) w[i] = 0;
+        for (int i = threadIdx.x; i < (mass ? 2 : 1) * ST_BINS; i += ST_THREADS) w[i] = 0;
         __syncthreads();
     }
     // adds a token to a histogram
@@ -391,11 +468,11 @@ struct SampleRow {
             atomicAdd(&s.word[0][bin], 1u);
             return;
         }
-        constexpr uint32_t mask = (1u << ST_LIMB) - 1;
-        const uint32_t lo = (uint32_t)weight & mask, mid = (uint32_t)(weight >> ST_LIMB) & mask, hi = (uint32_t)(weight >> (2 * ST_LIMB));
-        if (lo != 0) atomicAdd(&s.word[0][bin], lo);
-        if (mid != 0) atomicAdd(&s.word[1][bin], mid);
-        if (hi != 0) atomicAdd(&s.word[2][bin], hi);
+        // (one addition for most: a 64-bit one took several times as long)
+        const uint32_t lo = (uint32_t)weight;
+        if (weight == 0) return;
+        const uint32_t hi = (uint32_t)(weight >> 32) + (atomicAdd(&s.word[0][bin], lo) + lo < lo ? 1 : 0);
+        if (hi != 0) atomicAdd(&s.word[1][bin], hi);
     }
     // The bin in which the sums over the cluster's histograms reach goal(whole sum) (1 to the whole sum), the same in every CTA.
     template <typename G>
@@ -405,16 +482,29 @@ struct SampleRow {
         const int bins = ST_BINS / ranks, per = bins < ST_THREADS ? 1 : bins / ST_THREADS, at = rank * bins + threadIdx.x * per;
         const bool active = (int)threadIdx.x * per < bins;
         uint64_t mine[4] = {0, 0, 0, 0}, sum = 0;
-        if (active)
-            for (int r = 0; r < ranks; r++) {
-                const SampleShared* o = cl.map_shared_rank(&s, r);
+        if (active) {
+            // (all loads ahead of their sums: they come from other SMs)
+            if (per == 1) {
+                uint32_t lo[ST_MAX_CLUSTER], hi[ST_MAX_CLUSTER];
 #pragma unroll
-                for (int i = 0; i < 4; i++)
-                    if (i < per) {
-                        mine[i] += o->word[0][at + i];
-                        if (mass) mine[i] += ((uint64_t)o->word[1][at + i] << ST_LIMB) + ((uint64_t)o->word[2][at + i] << (2 * ST_LIMB));
-                    }
+                for (int r = 0; r < ST_MAX_CLUSTER; r++) {
+                    const SampleShared* o = cl.map_shared_rank(&s, min(r, ranks - 1));
+                    lo[r] = o->word[0][at];
+                    hi[r] = mass ? o->word[1][at] : 0;
+                }
+#pragma unroll
+                for (int r = 0; r < ST_MAX_CLUSTER; r++)
+                    if (r < ranks) mine[0] += (uint64_t)hi[r] << 32 | lo[r];
+            } else {
+#pragma unroll
+                for (int r = 0; r < 2; r++) {
+                    const SampleShared* o = cl.map_shared_rank(&s, min(r, ranks - 1));
+#pragma unroll
+                    for (int i = 0; i < 4; i++)
+                        if (i < per && r < ranks) mine[i] += (uint64_t)(mass ? o->word[1][at + i] : 0) << 32 | o->word[0][at + i];
+                }
             }
+        }
 #pragma unroll
         for (int i = 0; i < 4; i++) sum += mine[i];
         uint64_t total;
@@ -436,18 +526,16 @@ struct SampleRow {
         cl.sync();
         return s.found;
     }
-    // Goes over the CTA's tokens a run a thread: where f(number, value) says so, a token is listed, in no order.  Then the cluster's lists are gathered into the first CTA's;
+    // pass(list) goes over the CTA's tokens; those that it gives to list(number, value) are listed, in no order.  Then the cluster's lists are gathered into the first CTA's;
     // their tokens' number, or -1 where they are too many.  The lists lie over the histograms.  (A barrier of the cluster before the others' lists change.)
     template <typename F>
-    __device__ int gather(F f)
+    __device__ int gather(F pass)
     {
         if (threadIdx.x == 0) s.mine = 0;
         __syncthreads();
-        run([&](int i, float x) {
-            if (f(i, x)) {
-                const int at = atomicAdd(&s.mine, 1);
-                if (at < ST_LIST) s.list[at] = place(i, x);
-            }
+        pass([&](int i, float x) {
+            const int at = atomicAdd(&s.mine, 1);
+            if (at < ST_LIST) s.list[at] = place(i, x);
         });
         __syncthreads();
         if ((int)threadIdx.x < ranks) cl.map_shared_rank(&s, threadIdx.x)->listed[rank] = s.mine;
@@ -460,10 +548,9 @@ struct SampleRow {
         }
         if (!fits || sum > ST_LIST) return -1;
         if (rank == 0) {
-            for (int r = 1, at = s.listed[0]; r < ranks; at += s.listed[r++]) {
-                const uint64_t* from = cl.map_shared_rank(&s, r)->list;
-                for (int i = threadIdx.x; i < s.listed[r]; i += ST_THREADS) s.list[at + i] = from[i];
-            }
+            int r = 0, at = threadIdx.x;
+            while (r < ranks && at >= s.listed[r]) at -= s.listed[r++];
+            if (r > 0 && r < ranks) s.list[threadIdx.x] = cl.map_shared_rank(&s, r)->list[at];
             __syncthreads();
         }
         return sum;
@@ -473,59 +560,82 @@ struct SampleRow {
         for (int r = 0; r < ranks; r++) cl.map_shared_rank(&s, r)->cut = last;
     }
     // Among `count` listed tokens, in order: the one at which sums reach `rest`, told to the cluster.
-    __device__ void cut_list(bool mass, int count, uint64_t rest, const SampleWeight& weight)
+    __device__ void cut_list(bool mass, int count, uint64_t rest)
     {
         const int tid = threadIdx.x;
-        if (tid < count) {
-            const uint64_t v = s.list[tid];
-            s.sorted[st_rank(s.list, count, v)] = v;
-        }
-        __syncthreads();
+        st_sort(s.list, s.sorted, s.ranks, count);
         const uint64_t v = tid < count ? s.sorted[tid] : 0;
         const uint64_t w = tid >= count ? 0 : mass ? weight(st_unkey((uint32_t)(v >> 32))) : 1;
         uint64_t total;
         const uint64_t before = st_scan(w, s.scan, total);
         if (before < rest && rest <= before + w) tell(v);
     }
-    // Finds the token at which, in order, sums of those up to `limit` reach goal(their whole sum), by number or by weight.  sum: the thread's run's weights from `least` on of
-    // the bins before the token's, for the draw.
+    // Finds the token at which, in order, sums reach goal(their whole sum), by weight or by number.  few: of the tokens that reach `floor`, which are few.  sum, by weight: the
+    // thread's run's weights from `least` on of the bins before the token's, for the draw.
     template <typename G>
-    __device__ SampleCut select(bool mass, uint64_t limit, const SampleWeight& weight, uint64_t least, uint64_t& sum, G goal)
+    __device__ SampleCut select(bool mass, bool few, float floor, uint64_t least, uint64_t& sum, G goal)
     {
+        const int tid = threadIdx.x;
         clear(mass);
-        if (mass) {
-            pairs(threadIdx.x, ST_THREADS, vectors(), [&](int i, float x0, float x1) {
-                uint64_t w0, w1;
-                weight.two(x0, x1, w0, w1);
-                if (limit == ~0ull || place(i, x0) <= limit) put(true, coarse(x0), w0);
-                if (limit == ~0ull || place(i + 1, x1) <= limit) put(true, coarse(x1), w1);
-            });
+        if (few) {
+            above(tid, ST_THREADS, vectors(), floor, [&](int, float x) { put(mass, weight.coarse(x), mass ? weight(x) : 0); });
         } else {
-            all([&](int i, float x) {
-                if (limit == ~0ull || place(i, x) <= limit) put(false, coarse(x), 0);
+            pairs(tid, ST_THREADS, vectors(), [&](int, float x0, float x1) {
+                uint64_t w0 = 0, w1 = 0;
+                int b0, b1;
+                if (mass) {
+                    weight.two(x0, x1, w0, w1, b0, b1);
+                } else {
+                    b0 = weight.coarse(x0);
+                    b1 = weight.coarse(x1);
+                }
+                put(mass, b0, w0);
+                put(mass, b1, w1);
             });
         }
-        uint64_t target = 0;
-        SampleFound f = find(mass, [&](uint64_t whole) {
-            target = goal(whole);
-            return target;
+        uint64_t target = 0, whole = 0;
+        SampleFound f = find(mass, [&](uint64_t all) {
+            whole = all;
+            return target = goal(all);
         });
+        if (target > whole) return SampleCut{~0ull, -2};
         const int bin = f.bin;
-        if (!mass && bin == ST_BINS - 1) return SampleCut{limit, -1};      // weights of 2^-42 and less
+        if (bin > (ST_FIX + 1) * ST_OCTAVE) return SampleCut{~0ull, -1};      // it and all after it have no weight
         uint64_t rest = target - f.before;
         sum = 0;
         int count = 0;
-        count = gather([&](int i, float x) {
-            const int b = coarse(x);
-            if (b > bin || (limit != ~0ull && place(i, x) > limit)) return false;
-            if (b < bin) {
-                const uint64_t w = weight(x);
-                if (w >= least) sum += w;
+        const int begin = run_begin(tid), end = run_begin(tid + 1);
+        count = gather([&](auto list) {
+            if (few) {
+                above(begin, 1, end, floor, [&](int i, float x) {
+                    const int b = weight.coarse(x);
+                    if (b == bin) list(i, x);
+                    if (!mass || b >= bin) return;
+                    const uint64_t w = weight(x);
+                    if (w >= least) sum += w;
+                });
+            } else if (!mass) {
+                pairs(begin, 1, end, [&](int i, float x0, float x1) {
+                    if (weight.coarse(x0) == bin) list(i, x0);
+                    if (weight.coarse(x1) == bin) list(i + 1, x1);
+                });
+            } else {
+                auto body = [&](auto kept) {
+                    pairs(begin, 1, end, [&](int i, float x0, float x1) {
+                        uint64_t w0, w1;
+                        int b0, b1;
+                        weight.two(x0, x1, w0, w1, b0, b1);
+                        if (b0 == bin) list(i, x0);
+                        if (b1 == bin) list(i + 1, x1);
+                        sum += (b0 < bin ? kept(w0) : 0) + (b1 < bin ? kept(w1) : 0);
+                    });
+                };
+                if (least == 0) body([](uint64_t w) { return w; });
+                else body([least](uint64_t w) { return w >= least ? w : 0; });
             }
-            return b == bin;
         });
         if (count >= 0) {
-            if (rank == 0) cut_list(mass, count, rest, weight);
+            if (rank == 0) cut_list(mass, count, rest);
             cl.sync();
             return SampleCut{s.cut, bin};
         }
@@ -538,7 +648,7 @@ struct SampleRow {
             clear(mass);
             all([&](int i, float x) {
                 const uint32_t k = st_key(x);
-                if (coarse(x) == bin && (level == 0 || (k >> (shift + bits)) == prefix) && place(i, x) <= limit)
+                if (weight.coarse(x) == bin && (level == 0 || (k >> (shift + bits)) == prefix))
                     put(mass, (int)((k >> shift) & ((1u << bits) - 1)), mass ? weight(x) : 0);
             });
             f = find(mass, [&](uint64_t) { return rest; });
@@ -561,6 +671,25 @@ struct SampleRow {
             });
         cl.sync();
         return SampleCut{s.cut, -1};
+    }
+    // What lies after `last` becomes -infinity.
+    __device__ void erase(uint64_t last)
+    {
+        const float value = st_unkey((uint32_t)(last >> 32));
+        uint4* vecs = reinterpret_cast<uint4*>(vals - skew);
+        for (int v = threadIdx.x; v < vectors(); v += ST_THREADS) {
+            uint4 raw = vecs[v];
+            bool ties = false;
+            st_erase(raw, value, ties, vals);
+            if (ties) {
+                T* e = reinterpret_cast<T*>(&raw);
+#pragma unroll
+                for (int i = 0; i < VEC; i++)
+                    if (st_value(e[i]) == value && first + v * VEC - skew + i > (int)(uint32_t)last) e[i] = st_bits(-INFINITY, vals);
+            }
+            vecs[v] = raw;
+        }
+        __syncthreads();
     }
 };
 
@@ -615,7 +744,7 @@ __global__ void __launch_bounds__(ST_THREADS) ns_sample_tokens_kernel(const Samp
     if (tail + tid < n) take_one(tail + tid);
 #pragma unroll
     for (int i = 0; i < ST_TABLE / ST_THREADS; i++) {
-        s.table.fixed[tid + i * ST_THREADS] = power[i];
+        s.table.twice[tid + i * ST_THREADS] = 2 * power[i];
         s.table.value[tid + i * ST_THREADS] = (float)power[i];
     }
     // ---- the maximum
@@ -632,7 +761,6 @@ __global__ void __launch_bounds__(ST_THREADS) ns_sample_tokens_kernel(const Samp
     for (int r = 1; r < ranks; r++) max = fmaxf(max, s.max[r]);
 
     if (k <= 0 || k > p.vocab) k = p.vocab;
-    SampleRow<T> me{s, vals, n, first, skew, cl, rank, ranks, max, fminf(64.0f / temperature, 1e30f)};
     // Greedily, or nothing to choose from: every CTA sees the same and leaves, the first that has the maximum once it has found where.
     if (max == -INFINITY || !(temperature > 0.0f) || k == 1) {
         int owner = 0;
@@ -641,9 +769,8 @@ __global__ void __launch_bounds__(ST_THREADS) ns_sample_tokens_kernel(const Samp
             if (tid == 0) s.mine = n;
             __syncthreads();
             int at = n;
-            me.all([&](int i, float x) {
-                if (x == max) at = min(at, i);
-            });
+            for (int i = tid; i < n && at == n; i += ST_THREADS)
+                if (st_value(vals[i]) == max) at = i;
             if (at < n) atomicMin(&s.mine, at);
             __syncthreads();
             if (tid == 0) {
@@ -653,62 +780,103 @@ __global__ void __launch_bounds__(ST_THREADS) ns_sample_tokens_kernel(const Samp
         }
         return;
     }
+    if (max == INFINITY) {
+        // infinite tokens share everything: as zeros among tokens of -infinity
+        for (int i = tid; i < n; i += ST_THREADS) vals[i] = st_value(vals[i]) == INFINITY ? st_bits(0.0f, vals) : st_bits(-INFINITY, vals);
+        max = 0.0f;
+        __syncthreads();
+    }
     const SampleWeight weight(max, temperature, &s.table);
+    SampleRow<T> me{s, vals, n, first, skew, cl, rank, ranks, weight};
     uint64_t least = 0;
     if (min_p > 0.0f) least = (uint64_t)ceil((double)fminf(min_p, 1.0f) * (double)(1ull << ST_FIX));
 
-    // ---- few candidates
-    if (k <= ST_SORT_K && k < p.vocab) {
-        // from a sample: so much of it that k tokens hardly ever fail to be among those it stands for
-        int every = 1;
-        uint64_t need = k;
-        if (p.vocab > 1024 * ST_SAMPLE) {
-            every = ST_SAMPLE;
-            const float share = (float)k / ST_SAMPLE;
-            need = (uint64_t)(1.25f * share + 3.0f * sqrtf(share) + 4.0f);
-        }
-        me.clear(false);
-        for (int i = (every - first % every) % every + tid * every; i < n; i += ST_THREADS * every) me.put(false, me.coarse(st_value(vals[i])), 0);
-        const int bin = me.find(false, [&](uint64_t sample) { return need < sample ? need : sample; }).bin;
-        int count = 0;
-        // (about the tokens of those bins: as many as k of them is what counts)
-        const float near = max - ((float)bin + 0.5f) * (temperature * (1.0f / 64));
-        count = me.gather([&](int, float x) { return x >= near; });
-        if (count >= k) {
-            cl.sync();                     // the first CTA has the others' lists
-            if (rank != 0) return;
-            const SampleCuts cuts{k, top_p, p.u[row], least};
-            st_draw(s, count, cuts, weight, row, p);
-            return;
-        }
-        cl.sync();
-    }
-
-    // ---- cutoffs
+    // ---- the first k
     SampleCut cut{~0ull, -1};
     uint64_t sum = 0;
-    if (k < p.vocab) cut = me.select(false, cut.last, weight, least, sum, [&](uint64_t) { return (uint64_t)k; });
+    float floor = -INFINITY;
+    bool few = false;                      // few tokens reach `floor`, and all that are left do
+    if (k < p.vocab) {
+        auto list_few = [&](auto list) { me.above(me.run_begin(tid), 1, me.run_begin(tid + 1), floor, list); };
+        if (k <= ST_SORT_K || (p.vocab > 2048 * ST_SAMPLE && k <= p.vocab / 16)) {
+            // A value that about k tokens or some more reach, from a sample: so much of it that k hardly ever fail to be among those it stands for.
+            int every = 1;
+            uint64_t need = k;
+            if (p.vocab > 2048 * ST_SAMPLE) {
+                every = ST_SAMPLE;
+                const float share = (float)k / ST_SAMPLE;
+                need = (uint64_t)(1.25f * share + 3.0f * sqrtf(share) + 4.0f);
+            }
+            me.clear(false);
+            for (int i = (every - first % every) % every + tid * every; i < n; i += ST_THREADS * every) me.put(false, weight.coarse(st_value(vals[i])), 0);
+            const int bin = me.find(false, [&](uint64_t sample) { return need < sample ? need : sample; }).bin;
+            floor = fmaxf(max - ((float)bin + 1.0f) * (temperature * (0.69314718f / ST_OCTAVE)), -3e38f);
+            floor = __uint_as_float(__float_as_uint(floor) & 0xFFFF0000u);
+            few = true;
+        }
+        if (k <= ST_SORT_K) {
+            int count = 0;
+            count = me.gather(list_few);
+            if (count >= k) {
+                const SampleCuts cuts{k, top_p, p.u[row], least};
+                cl.sync();                 // the first CTA has the others' lists
+                if (rank != 0) return;
+                st_draw(s, count, cuts, weight, row, p);
+                return;
+            }
+            cl.sync();
+            few = count < 0;               // too many, or not enough
+        }
+        auto number = [&](uint64_t) { return (uint64_t)k; };
+        cut = me.select(false, few, floor, least, sum, number);
+        if (cut.bin == -2) {               // the guess was too high
+            cl.sync();
+            few = false;
+            cut = me.select(false, few, floor, least, sum, number);
+        }
+        if (cut.last != ~0ull) {
+            if (few && cut.bin >= 0) {
+                // what reaches the value of the last token and lies after it is among the CTA's part of the lists
+                if (tid < s.mine && s.list[tid] > cut.last) vals[(int)(uint32_t)s.list[tid] - first] = st_bits(-INFINITY, vals);
+                __syncthreads();
+            } else {
+                me.erase(cut.last);
+                few = k <= p.vocab / 16;
+            }
+            floor = st_unkey((uint32_t)(cut.last >> 32));
+            cut = SampleCut{~0ull, -1};
+        } else {
+            few = false;
+        }
+    }
+    // ---- of those, the first that have p of the weight
     if (top_p < 1.0f) {
         cl.sync();
-        cut = me.select(true, cut.last, weight, least, sum, [&](uint64_t whole) { return st_goal(top_p, whole); });
+        cut = me.select(true, few, floor, least, sum, [&](uint64_t whole) { return st_goal(top_p, whole); });
+        if (cut.bin < 0 && cut.last != ~0ull) {
+            me.erase(cut.last);
+            cut = SampleCut{~0ull, -1};
+        }
     }
 
     // ---- the draw: the weights of each thread's run
-    auto kept = [&](int i, float x) {
-        const uint64_t w = cut.last == ~0ull || me.place(i, x) <= cut.last ? weight(x) : 0;
-        return w >= least ? w : 0;
-    };
     if (cut.bin < 0) {
         sum = 0;
-        if (cut.last == ~0ull) {
-            me.pairs(me.run_begin(tid), 1, me.run_begin(tid + 1), [&](int, float x0, float x1) {
+        const int begin = me.run_begin(tid), end = me.run_begin(tid + 1);
+        auto sums = [&](auto kept) {
+            me.pairs(begin, 1, end, [&](int, float x0, float x1) {
                 uint64_t w0, w1;
                 weight.two(x0, x1, w0, w1);
-                sum += (w0 >= least ? w0 : 0) + (w1 >= least ? w1 : 0);
+                sum += kept(w0) + kept(w1);
             });
-        } else {
-            me.run([&](int i, float x) { sum += kept(i, x); });
-        }
+        };
+        if (few)
+            me.above(begin, 1, end, floor, [&](int, float x) {
+                const uint64_t w = weight(x);
+                if (w >= least) sum += w;
+            });
+        else if (least == 0) sums([](uint64_t w) { return w; });
+        else sums([least](uint64_t w) { return w >= least ? w : 0; });
     } else {
         // all but the cutoff's bin are in the sums: its tokens are this CTA's part of the lists
         s.extra[tid] = 0;
@@ -744,7 +912,11 @@ __global__ void __launch_bounds__(ST_THREADS) ns_sample_tokens_kernel(const Samp
     if (__syncthreads_or(mine)) {
         const int i = s.run_first * me.VEC - skew + tid;
         uint64_t w = 0, unused;
-        if (i >= 0 && i < n && i < s.run_end * me.VEC - skew) w = kept(i, st_value(vals[i]));
+        if (i >= 0 && i < n && i < s.run_end * me.VEC - skew) {
+            const float x = st_value(vals[i]);
+            w = weight(x);
+            if (w < least || (few && x < floor) || me.place(i, x) > cut.last) w = 0;
+        }
         const uint64_t at = s.run_before + st_scan(w, s.scan2, unused);
         if (at <= aim && aim < at + w) {
             p.ids[row] = first + i;
