@@ -31,6 +31,7 @@ constexpr int ST_MAX_CLUSTER = 8;
 constexpr int ST_FIX = 42;                 // weights are multiples of 2^-42: 2^20 of them fit 64 bits
 constexpr int ST_FAR = 45;                 // 2^-45 and less is no weight
 constexpr int ST_OCTAVE = 45;              // bins of the first histogram that halve the weight
+constexpr int ST_GUESS = ST_BINS / ST_THREADS;
 constexpr float ST_MAGIC = 12582912.0f;    // 1.5 * 2^23: the low bits of a sum with it are the rounded value
 constexpr int ST_TABLE = 1024;             // 2^(-i / 1024)
 constexpr int ST_LIST = ST_THREADS;         // candidates that are sorted: one a thread
@@ -95,7 +96,11 @@ struct alignas(16) SampleShared {
     int listed[ST_MAX_CLUSTER], mine;
     SampleTable table;
     uint64_t part[ST_MAX_CLUSTER], draw[ST_MAX_CLUSTER];       // of every CTA of the cluster, written between its barriers
-    uint64_t extra[ST_THREADS];            // of each thread's run
+    union {
+        uint64_t extra[ST_THREADS];        // of each thread's run
+        uint32_t guess[ST_THREADS];        // a histogram of a sample: of ST_GUESS bins of the first one
+    };
+    int guessed;
     uint64_t scan[ST_THREADS / 32], scan2[ST_THREADS / 32];
     float max[ST_MAX_CLUSTER], red[ST_THREADS / 32];
     SampleFound found;
@@ -747,6 +752,7 @@ __global__ void __launch_bounds__(ST_THREADS) ns_sample_tokens_kernel(const Samp
         s.table.twice[tid + i * ST_THREADS] = 2 * power[i];
         s.table.value[tid + i * ST_THREADS] = (float)power[i];
     }
+    s.guess[tid] = 0;
     // ---- the maximum
 #pragma unroll
     for (int o = 16; o > 0; o >>= 1) best = fmaxf(best, __shfl_xor_sync(0xffffffffu, best, o));
@@ -807,10 +813,18 @@ __global__ void __launch_bounds__(ST_THREADS) ns_sample_tokens_kernel(const Samp
                 const float share = (float)k / ST_SAMPLE;
                 need = (uint64_t)(1.25f * share + 3.0f * sqrtf(share) + 4.0f);
             }
-            me.clear(false);
-            for (int i = (every - first % every) % every + tid * every; i < n; i += ST_THREADS * every) me.put(false, weight.coarse(st_value(vals[i])), 0);
-            const int bin = me.find(false, [&](uint64_t sample) { return need < sample ? need : sample; }).bin;
-            floor = fmaxf(max - ((float)bin + 1.0f) * (temperature * (0.69314718f / ST_OCTAVE)), -3e38f);
+            for (int i = (every - first % every) % every + tid * every; i < n; i += ST_THREADS * every) atomicAdd(&s.guess[weight.coarse(st_value(vals[i])) / ST_GUESS], 1u);
+            cl.sync();
+            uint64_t in_bin = 0, sample;   // every CTA sums them all: that takes one barrier instead of three
+            uint32_t of[ST_MAX_CLUSTER];
+#pragma unroll
+            for (int r = 0; r < ST_MAX_CLUSTER; r++) of[r] = cl.map_shared_rank(&s, min(r, ranks - 1))->guess[tid];
+#pragma unroll
+            for (int r = 0; r < ST_MAX_CLUSTER; r++) in_bin += r < ranks ? of[r] : 0;
+            const uint64_t ahead = st_scan(in_bin, s.scan, sample), wanted = need < sample ? need : sample;
+            if (ahead < wanted && wanted <= ahead + in_bin) s.guessed = tid * ST_GUESS + ST_GUESS - 1;
+            __syncthreads();
+            floor = fmaxf(max - ((float)s.guessed + 1.0f) * (temperature * (0.69314718f / ST_OCTAVE)), -3e38f);
             floor = __uint_as_float(__float_as_uint(floor) & 0xFFFF0000u);
             few = true;
         }
@@ -819,9 +833,9 @@ __global__ void __launch_bounds__(ST_THREADS) ns_sample_tokens_kernel(const Samp
             count = me.gather(list_few);
             if (count >= k) {
                 const SampleCuts cuts{k, top_p, p.u[row], least};
-                cl.sync();                 // the first CTA has the others' lists
-                if (rank != 0) return;
-                st_draw(s, count, cuts, weight, row, p);
+                auto listed = cl.barrier_arrive();         // the first CTA has the others' lists
+                if (rank == 0) st_draw(s, count, cuts, weight, row, p);
+                cl.barrier_wait(static_cast<decltype(listed)&&>(listed));
                 return;
             }
             cl.sync();
