@@ -296,8 +296,9 @@ NS_API int ns_f32_history_push(ns_device_t dev, uint64_t ids, uint64_t history, 
  * ids[r] (int32) is the first token in the vocabulary's order at which the running sum of kept weights exceeds u[r] times their sum, u[r] in [0, 1);
  * probs[r] (float; probs may be 0) its weight over that sum.  A temperature that is not above 0 takes the first maximum.  NaN counts as -infinity; where all
  * are, ids[r] = -1 and probs[r] = 0.  temperature, top_p, min_p float [rows], top_k int32 [rows]: each may be 0, which leaves that step out (temperature: 1).
- * Weights are computed in 64 bits and summed exactly in units of 2^-44 (smaller ones are never drawn), so a row's token does not depend on the other
- * rows or their number.  vocab at most 380 000 floats or 760 000 bf16. */
+ * Weights are computed to 2^-33 of themselves, rounded to multiples of 2^-42 (a token of less is never drawn) and summed exactly, so a row's token does
+ * not depend on the other rows or their number.  Logits that are further apart than a float reaches count as infinitely far.  row_stride may be 0 (several draws
+ * from one row).  vocab at most 380 000 floats or 760 000 bf16. */
 NS_API int ns_sample_tokens(ns_device_t dev, uint64_t logits, int dtype, int64_t row_stride, int rows, int vocab, uint64_t temperature, uint64_t top_k,
                             uint64_t top_p, uint64_t min_p, uint64_t u, uint64_t ids, uint64_t probs);
 

@@ -244,7 +244,6 @@ __device__ __forceinline__ uint64_t st_fma2(uint64_t a, uint64_t b, uint64_t c)
     asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(y) : "l"(a), "l"(b), "l"(c));
     return y;
 }
-__device__ __forceinline__ uint64_t st_neg2(uint64_t a) { return a ^ 0x8000000080000000ull; }
 
 // a * b + c
 __device__ __forceinline__ uint64_t st_mad(int a, int b, uint64_t c)
@@ -277,7 +276,8 @@ struct SampleWeight {
     __device__ __forceinline__ void two(float x0, float x1, uint64_t& w0, uint64_t& w1, int& b0, int& b1) const
     {
         const uint64_t x = st_pair(x0, x1), m = st_pair(max, max), r2 = st_pair(rate, rate), magic = st_pair(ST_MAGIC, ST_MAGIC);
-        const uint64_t d = st_add2(m, st_neg2(x));
+        // (differences as products with -1: the sign of a pair would be two more integer operations)
+        const uint64_t minus = st_pair(-1.0f, -1.0f), minus_m = st_pair(-max, -max), d = st_fma2(x, minus, m);
         float p0, p1;
         st_split(st_mul2(d, r2), p0, p1);
         const uint64_t p = st_pair(limit(p0), limit(p1));
@@ -288,10 +288,10 @@ struct SampleWeight {
         b1 = bin(n1);
         w0 = w1 = 0;
         if (fminf(p0, p1) >= (float)ST_FAR) return;
-        // d + d_lo = max - x
-        const uint64_t back = st_add2(d, st_neg2(m)), d_lo = st_add2(st_add2(m, st_neg2(st_add2(d, st_neg2(back)))), st_neg2(st_add2(x, back)));
-        const uint64_t p_lo = st_fma2(d_lo, r2, st_fma2(d, st_pair(rate_lo, rate_lo), st_fma2(d, r2, st_neg2(p))));
-        const uint64_t r = st_add2(st_fma2(st_add2(ni, st_neg2(magic)), st_pair(-0.0009765625f, -0.0009765625f), p), p_lo);      // (the product and its sum are exact)
+        // d + d_lo = max - x; p + p_lo = its product with the rate
+        const uint64_t back = st_add2(d, minus_m), minus_d_lo = st_fma2(st_fma2(st_fma2(back, minus, d), minus, m), minus, st_add2(x, back));
+        const uint64_t e = st_add2(x, minus_m), minus_p_lo = st_fma2(minus_d_lo, r2, st_fma2(e, st_pair(rate_lo, rate_lo), st_fma2(e, r2, p)));
+        const uint64_t r = st_fma2(minus_p_lo, minus, st_fma2(st_add2(ni, st_pair(-ST_MAGIC, -ST_MAGIC)), st_pair(-0.0009765625f, -0.0009765625f), p));      // (the product and its sum are exact)
         const uint64_t q = st_mul2(r, st_fma2(r, st_fma2(r, st_pair(-0.055504109f, -0.055504109f), st_pair(0.24022651f, 0.24022651f)), st_pair(-0.69314718f, -0.69314718f)));
         float q0, q1;
         st_split(q, q0, q1);
@@ -973,8 +973,8 @@ extern "C" int ns_sample_tokens(ns_device_t h, uint64_t logits, int dtype, int64
     p.u = reinterpret_cast<const float*>(u);
     p.ids = reinterpret_cast<int32_t*>(ids);
     p.probs = reinterpret_cast<float*>(probs);
-    // CTAs a row: as many as leave room for two of them an SM (one has too few warps for the latency of its passes: 256 rows of 131 001 bf16 NNN us with two a row,
-    // NNN with four), and until the SMs are full or a thread has few tokens left.
+    // CTAs a row: as many as leave room for two of them an SM (one has too few warps for the latency of its passes: 256 rows of 131 001 bf16 182 us with two a row,
+    // 150 with four, 186 with eight), and until the SMs are full or a thread has few tokens left.
     int ranks = 1;
     auto each = [&](int r) { return ((vocab + r - 1) / r + 7) / 8 * 8; };
     while (ranks < ST_MAX_CLUSTER && (2 * st_bytes(each(ranks), size) > (size_t)most || ((int64_t)rows * ranks < d->sm_count && each(ranks) > 8 * ST_THREADS))) ranks *= 2;
