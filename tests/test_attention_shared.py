@@ -212,6 +212,33 @@ def test_scores_that_are_no_numbers(dev, dim, page, batch, prefix):
 
 
 @pytest.mark.gpu
+@pytest.mark.parametrize("bad", [0x7FC0, 0x7F80, 0xFF80])
+@pytest.mark.parametrize("dim,group,steps,batch,prefix", [(128, 2, 3, 2, 40), (64, 4, 7, 3, 0), (32, 1, 20, 2, 77), (128, 4, 2, 40, 2600), (64, 8, 5, 4, 0)])
+def test_a_later_token_of_the_call_does_not_reach_an_earlier_one(dev, dim, group, steps, batch, prefix, bad):
+    """Keys and values of a token that are no numbers: the tokens before it in the same call do not see it."""
+    for own in (steps, 37, 130):
+        s = Setup(dev, dim, 2, group, 16, batch, steps, prefix, [own] * batch)
+        s.upload()
+        clean = s.call()
+        s.check(clean)
+        for i in (1, steps - 1):               # the call's i-th token
+            for what in "kv":
+                kept = getattr(s, what).copy()
+                j = own - steps + i
+                getattr(s, what)[s.table[0][j // 16], 1, j % 16] = bad
+                s.upload()
+                got = s.call()
+                assert np.array_equal(got[1:], clean[1:]) and np.array_equal(got[0, :, :group], clean[0, :, :group])
+                with np.errstate(invalid="ignore"):
+                    want, tol = s.want()
+                assert (abs(values(got[0, :i]) - want[0, :i]) <= tol[0, :i]).all()
+                if bad == 0x7FC0:
+                    assert np.isnan(values(got[0, i:, group:])).all()
+                setattr(s, what, kept)
+        s.close()
+
+
+@pytest.mark.gpu
 @pytest.mark.parametrize("dim,page,batch,prefix", [(128, 16, 3, 100), (64, 64, 40, 500), (128, 32, 100, 1111), (32, 4, 4, 50), (128, 16, 40, 2600), (64, 8, 150, 1500), (128, 128, 64, 1600), (32, 16, 120, 3400)])
 def test_pages_outside_the_pool(dev, dim, page, batch, prefix):
     """Positions of a page that is none are left out and reported."""

@@ -104,6 +104,55 @@ def test_equal_logits(dev):
 
 
 @pytest.mark.gpu
+@pytest.mark.parametrize("dtype", [N.NS_F32, N.NS_BF16])
+@pytest.mark.parametrize("vocab", [16500, 50001])
+def test_large_tokens_at_regular_places(dev, vocab, dtype):
+    """The largest tokens all at every 8th place, none of them there, side by side, in order, many of one value: what a guess from a part of the row takes for more or for fewer
+    than there are."""
+    rng = np.random.default_rng(vocab)
+    places = [np.arange(0, 8 * 400, 8), np.arange(3, 3 + 8 * 400, 8), np.arange(100, 500), np.arange(vocab - 400, vocab), np.arange(0, 8 * 2000, 8)]
+    rows, xs = [], []
+    for where in places:
+        for high in (6.0, 0.5):
+            x = rng.standard_normal(vocab).astype(np.float32)
+            x[where] = high + rng.standard_normal(len(where)).astype(np.float32) * 0.5
+            xs.append(x)
+    xs.append(np.sort(rng.standard_normal(vocab).astype(np.float32)))
+    xs.append(xs[-1][::-1].copy())
+    xs.append(np.where(np.arange(vocab) % 8 == 0, 1.0, 0.0).astype(np.float32))
+    xs.append(np.where(np.arange(vocab) % 97 == 5, 3.0, -1.0).astype(np.float32))
+    base = np.stack(xs)
+    ks = [2, 20, 50, 128, 129, 300, 1000, vocab // 16, vocab // 16 + 1, vocab - 1]
+    x = np.repeat(base, len(ks), axis=0)
+    n = len(x)
+    bits, rounded = bf16(x)
+    x = rounded if dtype == N.NS_BF16 else x
+    k = np.tile(np.array(ks, np.int32), len(base))
+    for top_p, min_p, t in ((1.0, 0.0, 1.0), (0.9, 0.0, 0.7), (0.99, 0.05, 2.0)):
+        s = dict(temperature=np.full(n, t, np.float32), top_k=k, top_p=np.full(n, top_p, np.float32), min_p=np.full(n, min_p, np.float32), u=rng.random(n).astype(np.float32))
+        ids, probs = sample(dev, bits if dtype == N.NS_BF16 else x, dtype, n, vocab, vocab, s)
+        check(ids, probs, x, s)
+
+
+@pytest.mark.gpu
+def test_temperatures_and_logits_of_every_size(dev):
+    rng = np.random.default_rng(7)
+    vocab = 20000
+    xs, ts = [], []
+    for scale in (1e-38, 1e-20, 1.0, 1e20, 1e37):
+        for t in (1e-37, 1e-20, 1e-3, 1.0, 1e6, 1e20, 3e38, np.inf):
+            xs.append(rng.standard_normal(vocab).astype(np.float32) * np.float32(scale))
+            ts.append(t)
+    x = np.stack(xs)
+    n = len(x)
+    for k in (0, 30, 700):
+        for top_p in (1.0, 0.8):
+            s = dict(temperature=np.array(ts, np.float32), top_k=np.full(n, k, np.int32), top_p=np.full(n, top_p, np.float32), u=rng.random(n).astype(np.float32))
+            ids, probs = sample(dev, x, N.NS_F32, n, vocab, vocab, s)
+            check(ids, probs, x, s)
+
+
+@pytest.mark.gpu
 def test_values_that_are_no_numbers(dev):
     rng = np.random.default_rng(2)
     vocab = 5000
