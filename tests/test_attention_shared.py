@@ -125,7 +125,7 @@ CASES = [  # dim, kv heads, group, page, prefix, own positions of each sequence 
     (32, 1, 40, 16, 200, [20, 25], 1),              # groups of more heads than a tile has rows
     (128, 1, 2, 256, 900, [300, 20], 70),           # a portion of a prompt
     (64, 2, 3, 64, 3000, [90] * 50, 1),
-    # work enough for the tensor-core kernel: 800 000 products of 128 columns
+    # work enough for the tensor-core kernel, 1 000 000 products of 128 columns, and some a little short of it
     (128, 1, 8, 64, 2000, [40, 1] * 32, 1),         # 512 rows: two tiles
     (128, 2, 4, 16, 3333, [17] * 32, 1),            # 128 rows: the groups take turns
     (128, 4, 2, 8, 2600, [5, 60] * 20, 1),          # 80 rows
@@ -136,6 +136,12 @@ CASES = [  # dim, kv heads, group, page, prefix, own positions of each sequence 
     (32, 2, 8, 16, 4099, [5, 33] * 16, 1),          # heads of 32 columns lie two keys a row
     (32, 1, 16, 64, 3001, [20] * 70, 1),
     (32, 4, 2, 256, 5000, [3] * 20, 4),
+    (128, 2, 4, 16, 4001, [17] * 32, 1),            # 128 rows: the groups take turns
+    (128, 4, 2, 8, 3300, [5, 60] * 20, 1),          # 80 rows
+    (128, 1, 12, 64, 145, [1] * 600, 1),            # 7200 rows, two blocks
+    (32, 2, 8, 16, 8200, [5, 33] * 16, 1),
+    (32, 1, 16, 64, 3801, [20] * 70, 1),
+    (32, 4, 2, 256, 6600, [3] * 20, 4),
     (64, 1, 8, 16, 300, [], 1),                     # (filled in below: many sequences without pages of their own)
 ]
 
@@ -172,7 +178,8 @@ def test_padding_and_rows_that_see_nothing(dev, dim, page, batch):
 
 @pytest.mark.gpu
 @pytest.mark.parametrize("dim,kv,group,page,batch,prefix", [(128, 2, 4, 64, 5, 300), (64, 1, 2, 16, 3, 65), (32, 2, 4, 4, 4, 130), (128, 1, 4, 16, 64, 1000), (64, 1, 4, 32, 50, 77),
-                                                              (128, 1, 8, 16, 64, 1700), (64, 2, 8, 64, 40, 3001), (128, 2, 4, 64, 16, 6500), (128, 1, 8, 256, 60, 2050), (32, 2, 8, 16, 60, 3501), (32, 1, 8, 32, 120, 3333)])
+                                                              (128, 1, 8, 16, 64, 1700), (64, 2, 8, 64, 40, 3001), (128, 2, 4, 64, 16, 6500), (128, 1, 8, 256, 60, 2050), (32, 2, 8, 16, 60, 3501), (32, 1, 8, 32, 120, 3333), (128, 1, 8, 16, 64, 2001), (64, 2, 8, 64, 40, 3301), (128, 2, 4, 64, 16, 8000),
+                                                              (128, 1, 8, 256, 60, 2150), (32, 2, 8, 16, 60, 4400), (32, 1, 8, 32, 120, 4300)])
 def test_what_is_not_seen_does_not_count(dev, dim, kv, group, page, batch, prefix):
     """Behind the last position of the prefix and of every sequence, and in pages nobody names: NaN, infinities, the type's lowest value."""
     own = [1 + (7 * b) % 45 for b in range(batch)]
@@ -193,7 +200,8 @@ def test_what_is_not_seen_does_not_count(dev, dim, kv, group, page, batch, prefi
 
 
 @pytest.mark.gpu
-@pytest.mark.parametrize("dim,page,batch,prefix", [(128, 64, 2, 200), (64, 16, 40, 200), (128, 16, 70, 200), (32, 16, 5, 200), (128, 16, 70, 3000), (64, 64, 30, 14000), (32, 16, 250, 3300)])
+@pytest.mark.parametrize("dim,page,batch,prefix", [(128, 64, 2, 200), (64, 16, 40, 200), (128, 16, 70, 200), (32, 16, 5, 200), (128, 16, 70, 3000), (64, 64, 30, 14000), (32, 16, 250, 3300), (128, 16, 70, 3700),
+                                                    (64, 64, 30, 17200), (32, 16, 250, 4200)])
 def test_scores_that_are_no_numbers(dev, dim, page, batch, prefix):
     """A NaN among the keys a row sees makes the row NaN, and only the rows that see it; a value of NaN too."""
     for where in ("prefix", "own"):
@@ -239,7 +247,8 @@ def test_a_later_token_of_the_call_does_not_reach_an_earlier_one(dev, dim, group
 
 
 @pytest.mark.gpu
-@pytest.mark.parametrize("dim,page,batch,prefix", [(128, 16, 3, 100), (64, 64, 40, 500), (128, 32, 100, 1111), (32, 4, 4, 50), (128, 16, 40, 2600), (64, 8, 150, 1500), (128, 128, 64, 1600), (32, 16, 120, 3400)])
+@pytest.mark.parametrize("dim,page,batch,prefix", [(128, 16, 3, 100), (64, 64, 40, 500), (128, 32, 100, 1111), (32, 4, 4, 50), (128, 16, 40, 2600), (64, 8, 150, 1500), (128, 128, 64, 1600), (32, 16, 120, 3400),
+                                                    (128, 16, 40, 3300), (64, 8, 150, 1800), (128, 128, 64, 2100), (32, 16, 120, 4400)])
 def test_pages_outside_the_pool(dev, dim, page, batch, prefix):
     """Positions of a page that is none are left out and reported."""
     s = Setup(dev, dim, 2, 4, page, batch, 1, prefix, [60] * batch)
