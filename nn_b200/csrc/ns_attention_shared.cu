@@ -53,7 +53,10 @@ __global__ void __launch_bounds__(SH_THREADS, 3) ns_attention_shared_walk_kernel
     __shared__ uint32_t masks[SH_WARPS][SH_STAGES];
     __shared__ float2 fold[SH_WARPS][ROWS];
     // (beside the tensor-core kernel, which needs the whole of the SMs it has: what came before that has completed, and nothing here needs its results)
-    if (p.beside == nullptr) ns_pdl_wait();
+    if (p.beside == nullptr) {
+        ns_pdl_wait();
+        ns_pdl_trigger();
+    }
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
 
     // ---- which rows and which keys
@@ -466,7 +469,10 @@ int launch_shared(NsDevice* d, const SharedParams& p, int row_tile)
         const int64_t rows = (int64_t)p.batch * p.steps * p.heads;
         const bool many = p.prefix_parts + p.own_parts > 16 && rows <= 1024;
         auto fold = many ? ns_attention_shared_fold_kernel<DH, 8> : ns_attention_shared_fold_kernel<DH, 1>;
-        NS_CUDA(ns_launch_plain(fold, dim3((unsigned)(many ? rows : (rows + 7) / 8)), dim3(256), 0, d->stream, p));
+        const dim3 grid((unsigned)(many ? rows : (rows + 7) / 8));
+        // (early behind the walking kernel alone: 0.3 us of 6.5; where that runs beside the other one, its CTAs are in the way: 37.1 us became 38.1)
+        if (p.beside == nullptr) NS_CUDA(ns_launch_pdl(fold, grid, dim3(256), 0, d->stream, p));
+        else NS_CUDA(ns_launch_plain(fold, grid, dim3(256), 0, d->stream, p));
     }
     return NS_OK;
 }
