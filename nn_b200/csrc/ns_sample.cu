@@ -645,10 +645,11 @@ struct SampleRow {
             return SampleCut{s.cut, bin};
         }
         // too many: the key by its bits, then the token by its number among the key's
+        constexpr int LEVELS = sizeof(T) == 2 ? 2 : 3, LOW = sizeof(T) == 2 ? 16 : 0;
         uint32_t prefix = 0;
 #pragma unroll 1
-        for (int level = 0; level < 3; level++) {
-            const int shift = level == 0 ? 21 : level == 1 ? 10 : 0, bits = level == 2 ? 10 : 11;
+        for (int level = 0; level < LEVELS; level++) {
+            const int shift = level == 0 ? 21 : level == LEVELS - 1 ? LOW : 10, bits = level == 0 ? 11 : level == 1 ? 21 - shift : 10;
             cl.sync();
             clear(mass);
             all([&](int i, float x) {
@@ -660,6 +661,7 @@ struct SampleRow {
             rest -= f.before;
             prefix = (prefix << bits) | (uint32_t)f.bin;
         }
+        if (LOW != 0) prefix = prefix << LOW | ((prefix >> 15) != 0 ? 0u : 0xFFFFu);        // (the lower half of a bf16's key)
         if (mass) {
             const uint64_t w = weight(st_unkey(prefix));
             rest = (rest + w - 1) / w;
