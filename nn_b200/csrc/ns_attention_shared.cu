@@ -529,13 +529,15 @@ extern "C" int ns_attention_shared(ns_device_t h, ns_kv_cache_t cache, uint64_t 
     p.own_tiles = (steps * p.group + row_tile - 1) / row_tile;
     // Parts by position, of 64 keys at least and 64 of them at most, alike for prefix and own pages: as short as leaves all CTAs of the walking kernel on the SMs at once (three an SM with
     // 128 columns, four with fewer, one less with 16 rows).  Parts for four CTAs an SM from the prefix and as many from the own pages: 16 sequences of 500 positions, 4 query heads for each of 8, over 500
-    // 19.3 us, so 13.0; 8 of 2000 over 2000 24.3, 18.1; 8 x 5 x 16 heads of 64 columns, 300 over 2500, 18.4, 14.8; 4 of 500 over 4000 16.6, 12.5.
+    // 19.3 us, so 13.0; 8 of 2000 over 2000 24.3, 18.1; 8 x 5 x 16 heads of 64 columns, 300 over 2500, 18.4, 14.8; 4 of 500 over 4000 16.6, 12.5.  But no longer than a quarter more than
+    // the keys of all divided by so many CTAs: where the own pages' alone are more than that, a prefix in one part would end long after them.
     const int64_t prefix_keys = tiles ? 0 : (int64_t)prefix_pages * c.page_size, own_keys = (int64_t)max_pages * c.page_size, most = prefix_keys > own_keys ? prefix_keys : own_keys;
     const int64_t prefix_ctas = (int64_t)p.prefix_tiles * c.heads, own_ctas = max_pages > 0 ? (int64_t)batch * p.own_tiles * c.heads : 0;
     const int64_t wave = (int64_t)d->sm_count * (tiles ? 4 : (c.head_dim == 128 ? 3 : 4) - (row_tile == 16 ? 1 : 0));
     auto parts = [&](int64_t keys, int64_t length) { return keys == 0 ? 0 : (keys + length - 1) / length; };
+    const int64_t enough = (prefix_ctas * prefix_keys + own_ctas * own_keys) / (wave * 4 / 5);
     int64_t length = most <= 64 * 64 ? 64 : (most + 4095) / 4096 * 64;
-    while (length < most && prefix_ctas * parts(prefix_keys, length) + own_ctas * parts(own_keys, length) > wave) length += length / 512 * 64 + 64;
+    while (length < most && length < enough && prefix_ctas * parts(prefix_keys, length) + own_ctas * parts(own_keys, length) > wave) length += length / 512 * 64 + 64;
     if (!tiles) p.prefix_parts = (int)parts(prefix_keys, length);
     p.own_parts = (int)parts(own_keys, length);
     const int n_parts = p.prefix_parts + p.own_parts;

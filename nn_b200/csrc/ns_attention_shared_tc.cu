@@ -643,11 +643,11 @@ bool ns_attention_shared_tiles_fit(const NsDevice* d, const SharedParams& s, int
     // the scaled ones
     if (s.page_shift < (head_dim == 32 ? 4 : 3) || !(scale > 0.0f) || s.prefix_pages == 0) return false;
     // Little to multiply is the walking kernel's, which starts at once; so is what few rows have to read of long keys, which it has on their way from more places.  Both sides of the
-    // line, us, this kernel's way and the other's (rows of a key/value head x heads x keys x columns): 32 x 8 x 2000 x 128 15.2, 16.0; 64 x 2 x 8000 x 128 19.5, 21.2; 128 x 8 x 2000 x 128 20.7,
-    // 28.6; 64 x 8 x 2000 x 64 14.2, 14.9; 64 x 1 x 8000 x 128 15.9, 15.7; 256 x 2 x 2000 x 64 16.9, 14.9;
-    // 128 x 2 x 3333 x 128 22.5, 19.1; 40 x 16 x 2500 x 64 20.6, 18.5; 480 x 1 x 2050 x 128 25.4, 22.2; 64 x 8 x 2000 x 128 17.5, 21.9; 128 x 16 x 1000 x 64 22.3, 27.8; 8 x 8 x 8000 x 128 23.7, 15.8; 16 x 16 x 8000 x 128 32.6, 30.2.
+    // line, us, this kernel's way and the other's (rows of a key/value head x heads x keys x columns): 128 x 2 x 3333 x 128 22.6, 15.8; 64 x 8 x 2000 x 128 17.5, 17.2; 64 x 16 x 2500 x 64 21.0,
+    // 18.3; 256 x 4 x 1600 x 128 24.8, 20.7; 256 x 8 x 700 x 128 20.0, 23.0; 256 x 2 x 4000 x 128 21.6, 23.2; 128 x 8 x 2500 x 128 27.2, 32.3; 64 x 16 x 5000 x 64 24.6, 27.9; 24 x 8 x 16000 x 128
+    // 31.8, 33.6; 20 x 32 x 4000 x 128 42.0, 36.4; 16 x 16 x 8000 x 128 32.6, 30.2.
     const double work = (double)s.batch * s.steps * s.heads * ((double)s.prefix_pages * (1 << s.page_shift)) * head_dim;
-    if (work < ((int64_t)s.batch * s.steps * s.group >= 24 ? 1e6 : 4e6) * 128) return false;
+    if (work < ((int64_t)s.batch * s.steps * s.group >= 24 ? 1.7e6 : 4e6) * 128) return false;
     TileParams p;
     tile_plan(d, s, p);
     *parts = p.parts * (p.turns ? 2 : 1);

@@ -125,7 +125,7 @@ CASES = [  # dim, kv heads, group, page, prefix, own positions of each sequence 
     (32, 1, 40, 16, 200, [20, 25], 1),              # groups of more heads than a tile has rows
     (128, 1, 2, 256, 900, [300, 20], 70),           # a portion of a prompt
     (64, 2, 3, 64, 3000, [90] * 50, 1),
-    # work enough for the tensor-core kernel, 1 000 000 products of 128 columns, and some a little short of it
+    # work enough for the tensor-core kernel, 1 700 000 products of 128 columns, and some short of it
     (128, 1, 8, 64, 2000, [40, 1] * 32, 1),         # 512 rows: two tiles
     (128, 2, 4, 16, 3333, [17] * 32, 1),            # 128 rows: the groups take turns
     (128, 4, 2, 8, 2600, [5, 60] * 20, 1),          # 80 rows
@@ -142,6 +142,16 @@ CASES = [  # dim, kv heads, group, page, prefix, own positions of each sequence 
     (32, 2, 8, 16, 8200, [5, 33] * 16, 1),
     (32, 1, 16, 64, 3801, [20] * 70, 1),
     (32, 4, 2, 256, 6600, [3] * 20, 4),
+    (128, 1, 8, 64, 3500, [40, 1] * 32, 1),
+    (128, 2, 4, 16, 7000, [17] * 32, 1),
+    (128, 4, 2, 8, 5500, [5, 60] * 20, 1),
+    (64, 2, 8, 32, 7000, [33] * 33, 1),
+    (64, 8, 1, 128, 7000, [9, 200] * 16, 2),
+    (128, 1, 3, 256, 2050, [70] * 60, 5),
+    (128, 1, 12, 64, 250, [1] * 600, 1),
+    (32, 2, 8, 16, 13500, [5, 33] * 16, 1),
+    (32, 1, 16, 64, 6200, [20] * 70, 1),
+    (32, 4, 2, 256, 11000, [3] * 20, 4),
     (64, 1, 8, 16, 300, [], 1),                     # (filled in below: many sequences without pages of their own)
 ]
 
@@ -179,7 +189,8 @@ def test_padding_and_rows_that_see_nothing(dev, dim, page, batch):
 @pytest.mark.gpu
 @pytest.mark.parametrize("dim,kv,group,page,batch,prefix", [(128, 2, 4, 64, 5, 300), (64, 1, 2, 16, 3, 65), (32, 2, 4, 4, 4, 130), (128, 1, 4, 16, 64, 1000), (64, 1, 4, 32, 50, 77),
                                                               (128, 1, 8, 16, 64, 1700), (64, 2, 8, 64, 40, 3001), (128, 2, 4, 64, 16, 6500), (128, 1, 8, 256, 60, 2050), (32, 2, 8, 16, 60, 3501), (32, 1, 8, 32, 120, 3333), (128, 1, 8, 16, 64, 2001), (64, 2, 8, 64, 40, 3301), (128, 2, 4, 64, 16, 8000),
-                                                              (128, 1, 8, 256, 60, 2150), (32, 2, 8, 16, 60, 4400), (32, 1, 8, 32, 120, 4300)])
+                                                              (128, 1, 8, 256, 60, 2150), (32, 2, 8, 16, 60, 4400), (32, 1, 8, 32, 120, 4300), (128, 1, 8, 16, 64, 3500), (64, 2, 8, 64, 40, 5500),
+                                                              (128, 2, 4, 64, 16, 14000), (128, 1, 8, 256, 60, 3700), (32, 2, 8, 16, 60, 7300), (32, 1, 8, 32, 120, 7300)])
 def test_what_is_not_seen_does_not_count(dev, dim, kv, group, page, batch, prefix):
     """Behind the last position of the prefix and of every sequence, and in pages nobody names: NaN, infinities, the type's lowest value."""
     own = [1 + (7 * b) % 45 for b in range(batch)]
@@ -201,7 +212,7 @@ def test_what_is_not_seen_does_not_count(dev, dim, kv, group, page, batch, prefi
 
 @pytest.mark.gpu
 @pytest.mark.parametrize("dim,page,batch,prefix", [(128, 64, 2, 200), (64, 16, 40, 200), (128, 16, 70, 200), (32, 16, 5, 200), (128, 16, 70, 3000), (64, 64, 30, 14000), (32, 16, 250, 3300), (128, 16, 70, 3700),
-                                                    (64, 64, 30, 17200), (32, 16, 250, 4200)])
+                                                    (64, 64, 30, 17200), (32, 16, 250, 4200), (128, 16, 70, 6200), (64, 64, 30, 29000), (32, 16, 250, 7000)])
 def test_scores_that_are_no_numbers(dev, dim, page, batch, prefix):
     """A NaN among the keys a row sees makes the row NaN, and only the rows that see it; a value of NaN too."""
     for where in ("prefix", "own"):
@@ -221,7 +232,7 @@ def test_scores_that_are_no_numbers(dev, dim, page, batch, prefix):
 
 @pytest.mark.gpu
 @pytest.mark.parametrize("bad", [0x7FC0, 0x7F80, 0xFF80])
-@pytest.mark.parametrize("dim,group,steps,batch,prefix", [(128, 2, 3, 2, 40), (64, 4, 7, 3, 0), (32, 1, 20, 2, 77), (128, 4, 2, 40, 2600), (64, 8, 5, 4, 0)])
+@pytest.mark.parametrize("dim,group,steps,batch,prefix", [(128, 2, 3, 2, 40), (64, 4, 7, 3, 0), (32, 1, 20, 2, 77), (128, 4, 2, 40, 2600), (128, 4, 2, 40, 2900), (64, 8, 5, 4, 0)])
 def test_a_later_token_of_the_call_does_not_reach_an_earlier_one(dev, dim, group, steps, batch, prefix, bad):
     """Keys and values of a token that are no numbers: the tokens before it in the same call do not see it."""
     for own in (steps, 37, 130):
@@ -248,7 +259,8 @@ def test_a_later_token_of_the_call_does_not_reach_an_earlier_one(dev, dim, group
 
 @pytest.mark.gpu
 @pytest.mark.parametrize("dim,page,batch,prefix", [(128, 16, 3, 100), (64, 64, 40, 500), (128, 32, 100, 1111), (32, 4, 4, 50), (128, 16, 40, 2600), (64, 8, 150, 1500), (128, 128, 64, 1600), (32, 16, 120, 3400),
-                                                    (128, 16, 40, 3300), (64, 8, 150, 1800), (128, 128, 64, 2100), (32, 16, 120, 4400)])
+                                                    (128, 16, 40, 3300), (64, 8, 150, 1800), (128, 128, 64, 2100), (32, 16, 120, 4400),
+                                                    (128, 16, 40, 5500), (64, 8, 150, 2950), (128, 128, 64, 3400), (32, 16, 120, 7300)])
 def test_pages_outside_the_pool(dev, dim, page, batch, prefix):
     """Positions of a page that is none are left out and reported."""
     s = Setup(dev, dim, 2, 4, page, batch, 1, prefix, [60] * batch)

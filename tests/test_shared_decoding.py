@@ -111,7 +111,7 @@ class Step:
 
 
 @pytest.mark.gpu
-@pytest.mark.parametrize("batch,prompt,dim,group,page", [(3, 70, 64, 3, 16), (40, 2600, 128, 4, 64), (130, 300, 32, 1, 4), (24, 5000, 64, 8, 128), (40, 3300, 128, 4, 64), (28, 5000, 64, 8, 128)])
+@pytest.mark.parametrize("batch,prompt,dim,group,page", [(3, 70, 64, 3, 16), (40, 2600, 128, 4, 64), (130, 300, 32, 1, 4), (24, 5000, 64, 8, 128), (40, 3300, 128, 4, 64), (28, 5000, 64, 8, 128), (40, 5500, 128, 4, 64), (28, 8000, 64, 8, 128)])
 def test_continuations_of_one_prompt(dev, batch, prompt, dim, group, page):
     steps = 20
     s = Step(dev, batch, prompt, steps, dim=dim, group=group, page=page)
