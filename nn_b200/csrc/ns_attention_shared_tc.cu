@@ -645,9 +645,10 @@ bool ns_attention_shared_tiles_fit(const NsDevice* d, const SharedParams& s, int
     // Little to multiply is the walking kernel's, which starts at once; so is what few rows have to read of long keys, which it has on their way from more places.  Both sides of the
     // line, us, this kernel's way and the other's (rows of a key/value head x heads x keys x columns): 128 x 2 x 3333 x 128 22.6, 15.8; 64 x 8 x 2000 x 128 17.5, 17.2; 64 x 16 x 2500 x 64 21.0,
     // 18.3; 256 x 4 x 1600 x 128 24.8, 20.7; 256 x 8 x 700 x 128 20.0, 23.0; 256 x 2 x 4000 x 128 21.6, 23.2; 128 x 8 x 2500 x 128 27.2, 32.3; 64 x 16 x 5000 x 64 24.6, 27.9; 24 x 8 x 16000 x 128
-    // 31.8, 33.6; 20 x 32 x 4000 x 128 42.0, 36.4; 16 x 16 x 8000 x 128 32.6, 30.2.
-    const double work = (double)s.batch * s.steps * s.heads * ((double)s.prefix_pages * (1 << s.page_shift)) * head_dim;
-    if (work < ((int64_t)s.batch * s.steps * s.group >= 24 ? 1.7e6 : 4e6) * 128) return false;
+    // 31.8, 33.6; 20 x 32 x 4000 x 128 42.0, 36.4; 20 x 16 x 16000 x 128 45.7, 54.8; 16 x 32 x 16000 x 128 67.6, 62.8; 8 x 8 x 64000 x 128 64.0, 51.3.
+    const int64_t rows = (int64_t)s.batch * s.steps * s.group;
+    const double work = (double)rows * s.kv_heads * ((double)s.prefix_pages * (1 << s.page_shift)) * head_dim;
+    if (rows <= 16 || work < (rows >= 24 ? 1.7e6 : 4e6) * 128) return false;
     TileParams p;
     tile_plan(d, s, p);
     *parts = p.parts * (p.turns ? 2 : 1);
