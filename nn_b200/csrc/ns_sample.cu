@@ -11,8 +11,9 @@
 // definition's.)
 //
 // A cluster of 1 to 8 CTAs holds a row in shared memory; it is read from global memory once.  What remains costs passes over shared memory:
-//   - A top-k of up to ST_SORT_K: a histogram of every 8th token over (max - x) / T, 45 bins to each halving of the weight, names a cutoff that hardly ever fails to leave k candidates and leaves
-//     few more; they are gathered into one CTA, sorted (value, then index), cut by all three rules, sorted by index and drawn from.
+//   - A top-k of up to ST_WIDE_K: a histogram of every 8th token over (max - x) / T, 45 bins to each halving of the weight, names a cutoff that hardly ever fails to leave k candidates and
+//     leaves few more; they are gathered into one CTA.  Few are sorted (value, then index), cut by all three rules, sorted by index and drawn from; of more, the three places (of the
+//     k-th token, of p of the weight, of u of what is left) are found by a histogram and the tokens of one bin each.  (64 rows of 32 000 in turn 34.9 us with cutoffs of the whole cluster, so 27.1.)
 //   - Else cutoffs are found one after the other: a histogram, by number (from such a cutoff on) or by weight, names the bin in which a cutoff lies, and that bin's tokens
 //     alone are gathered and sorted (or, where they are too many, counted by the bits of x, 11 at a time).  The draw is then one more pass over the row, or, after a
 //     cutoff by weight, the sums of the pass that gathered.
@@ -35,7 +36,9 @@ constexpr int ST_GUESS = ST_BINS / ST_THREADS;
 constexpr float ST_MAGIC = 12582912.0f;    // 1.5 * 2^23: the low bits of a sum with it are the rounded value
 constexpr int ST_TABLE = 1024;             // 2^(-i / 1024)
 constexpr int ST_LIST = ST_THREADS;         // candidates that are sorted: one a thread
-constexpr int ST_SORT_K = 128;             // the largest top-k whose candidates they are
+constexpr int ST_SORT_K = 128;             // a top-k whose candidates are looked for in a short vocabulary too
+constexpr int ST_WIDE = 4 * ST_LIST;       // candidates that one CTA cuts with histograms of its own: four a thread
+constexpr int ST_WIDE_K = 1024;            // the largest top-k whose candidates one CTA takes
 constexpr int ST_SAMPLE = 8;               // its cutoff is guessed from every 8th token
 constexpr uint32_t ST_NO_CUT = 0xFFFFFFFFu;
 
@@ -91,6 +94,9 @@ struct alignas(16) SampleShared {
             __align__(16) uint64_t list[ST_LIST];        // candidates: key, index
             uint64_t sorted[ST_LIST], weights[ST_LIST];
             int ranks[ST_THREADS];
+        };
+        struct {
+            uint64_t wide[ST_WIDE];
         };
     };
     int listed[ST_MAX_CLUSTER], mine;
@@ -391,6 +397,110 @@ __device__ void st_draw(SampleShared& s, int count, const SampleCuts& cuts, cons
     }
 }
 
+// What one CTA needs to cut up to ST_WIDE candidates; it lies over the CTA's tokens.
+struct SampleNarrow {
+    uint32_t lo[ST_THREADS], hi[ST_THREADS];           // a histogram of amounts
+    uint64_t list[ST_LIST], sorted[ST_LIST];           // a bin's candidates
+    int ranks[ST_THREADS];
+    uint64_t before, key;
+    int found, count;
+};
+
+// st_draw for the candidates in s.wide, in no order, four a thread.  Three places are looked for in the same way: the key at which, in the keys' order, sums of amounts reach a
+// goal -- the k-th token, the one at which p of their weight is reached, and, with what is left in the order of the vocabulary, the drawn one.
+__device__ void st_draw_wide(SampleShared& s, SampleNarrow& m, int count, const SampleCuts& cuts, const SampleWeight& weight, int row, const SampleArgs& p)
+{
+    const int tid = threadIdx.x, shift = max(0, 32 - __clz(p.vocab) - 9);
+    uint64_t key[4], v[4], total = 0, last = ~0ull;
+    uint32_t live = 0;                                 // of the four, those that are left
+    int bin[4];                                        // a monotone function of the key
+    auto weigh = [&](uint64_t k) { return weight(st_unkey((uint32_t)(k >> 32))); };
+#pragma unroll
+    for (int i = 0; i < 4; i++) {
+        const int at = tid + i * ST_THREADS;
+        key[i] = at < count ? s.wide[at] : ~0ull;
+        live |= at < count ? 1u << i : 0;
+    }
+#pragma unroll
+    for (int i = 0; i < 4; i += 2) {
+        weight.two(st_unkey((uint32_t)(key[i] >> 32)), st_unkey((uint32_t)(key[i + 1] >> 32)), v[i], v[i + 1], bin[i], bin[i + 1]);
+        bin[i] /= ST_BINS / ST_THREADS;
+        bin[i + 1] /= ST_BINS / ST_THREADS;
+    }
+#pragma unroll 1
+    for (int step = 0; step < 3; step++) {
+        if (step == 1 && !(cuts.top_p < 1.0f)) continue;
+        uint64_t goal = (uint64_t)cuts.k;
+        auto amount = [&](int i) -> uint64_t { return (live >> i & 1) == 0 ? 0 : step == 0 ? 1 : v[i]; };
+#pragma unroll
+        for (int i = 0; i < 4; i++) {
+            if (key[i] > last || (step == 2 && v[i] < cuts.least)) live &= ~(1u << i);
+            if (step == 2) {
+                bin[i] = min((int)((uint32_t)key[i] >> shift), ST_THREADS - 1);
+                key[i] = key[i] << 32 | (uint32_t)(tid + i * ST_THREADS);
+            }
+        }
+        if (step > 0) {
+            st_scan(amount(0) + amount(1) + amount(2) + amount(3), s.scan2, total);
+            goal = step == 1 ? st_goal(cuts.top_p, total) : st_aim(cuts.u, total) + 1;
+        }
+        m.lo[tid] = m.hi[tid] = 0;
+        if (tid == 0) m.count = 0;
+        __syncthreads();
+#pragma unroll
+        for (int i = 0; i < 4; i++)
+            if (amount(i) != 0) {
+                const uint32_t lo = (uint32_t)amount(i), hi = (uint32_t)(amount(i) >> 32) + (atomicAdd(&m.lo[bin[i]], lo) + lo < lo ? 1 : 0);
+                if (hi != 0) atomicAdd(&m.hi[bin[i]], hi);
+            }
+        __syncthreads();
+        const uint64_t mine = (uint64_t)m.hi[tid] << 32 | m.lo[tid];
+        uint64_t all;
+        const uint64_t before = st_scan(mine, s.scan, all);
+        if (before < goal && goal <= before + mine) {
+            m.found = tid;
+            m.before = before;
+        }
+        __syncthreads();
+#pragma unroll
+        for (int i = 0; i < 4; i++)
+            if (amount(i) != 0 && bin[i] == m.found) {
+                const int at = atomicAdd(&m.count, 1);
+                if (at < ST_LIST) m.list[at] = key[i];
+            }
+        __syncthreads();
+        const int listed = m.count;
+        if (listed <= ST_LIST) {
+            st_sort(m.list, m.sorted, m.ranks, listed);
+            const uint64_t k = tid < listed ? m.sorted[tid] : 0, of = tid >= listed ? 0 : step == 0 ? 1 : weigh(step == 1 ? k : s.wide[(uint32_t)k]);
+            const uint64_t ahead = m.before + st_scan(of, s.scan2, all);
+            if (ahead < goal && goal <= ahead + of) m.key = k;
+        } else {
+            // more than can be sorted: by halves
+            uint64_t least = 0, most = ~0ull;
+            while (least < most) {
+                const uint64_t middle = least + (most - least) / 2;
+                uint64_t sum = 0;
+#pragma unroll
+                for (int i = 0; i < 4; i++) sum += key[i] <= middle ? amount(i) : 0;
+                __syncthreads();
+                st_scan(sum, s.scan2, all);
+                if (all >= goal) most = middle;
+                else least = middle + 1;
+            }
+            if (tid == 0) m.key = least;
+        }
+        __syncthreads();
+        last = m.key;
+    }
+#pragma unroll
+    for (int i = 0; i < 4; i++)
+        if (key[i] == last && (live >> i & 1) != 0) {
+            p.ids[row] = (int)(last >> 32);
+            if (p.probs != nullptr) p.probs[row] = (float)((double)v[i] / (double)total);
+        }
+}
+
 template <typename T>
 struct SampleRow {
     static constexpr int VEC = 16 / sizeof(T);
@@ -533,14 +643,14 @@ struct SampleRow {
     }
     // pass(list) goes over the CTA's tokens; those that it gives to list(number, value) are listed, in no order.  Then the cluster's lists are gathered into the first CTA's;
     // their tokens' number, or -1 where they are too many.  The lists lie over the histograms.  (A barrier of the cluster before the others' lists change.)
-    template <typename F>
+    template <int MOST = ST_LIST, typename F>
     __device__ int gather(F pass)
     {
         if (threadIdx.x == 0) s.mine = 0;
         __syncthreads();
         pass([&](int i, float x) {
             const int at = atomicAdd(&s.mine, 1);
-            if (at < ST_LIST) s.list[at] = place(i, x);
+            if (at < MOST) s.wide[at] = place(i, x);
         });
         __syncthreads();
         if ((int)threadIdx.x < ranks) cl.map_shared_rank(&s, threadIdx.x)->listed[rank] = s.mine;
@@ -548,14 +658,16 @@ struct SampleRow {
         int sum = 0;
         bool fits = true;
         for (int r = 0; r < ranks; r++) {
-            fits = fits && s.listed[r] <= ST_LIST;
+            fits = fits && s.listed[r] <= MOST;
             sum += s.listed[r];
         }
-        if (!fits || sum > ST_LIST) return -1;
+        if (!fits || sum > MOST) return -1;
         if (rank == 0) {
-            int r = 0, at = threadIdx.x;
-            while (r < ranks && at >= s.listed[r]) at -= s.listed[r++];
-            if (r > 0 && r < ranks) s.list[threadIdx.x] = cl.map_shared_rank(&s, r)->list[at];
+            for (int i = threadIdx.x; i < sum; i += ST_THREADS) {
+                int r = 0, at = i;
+                while (at >= s.listed[r]) at -= s.listed[r++];
+                if (r > 0) s.wide[i] = cl.map_shared_rank(&s, r)->wide[at];
+            }
             __syncthreads();
         }
         return sum;
@@ -805,7 +917,6 @@ __global__ void __launch_bounds__(ST_THREADS) ns_sample_tokens_kernel(const Samp
     float floor = -INFINITY;
     bool few = false;                      // few tokens reach `floor`, and all that are left do
     if (k < p.vocab) {
-        auto list_few = [&](auto list) { me.above(me.run_begin(tid), 1, me.run_begin(tid + 1), floor, list); };
         if (k <= ST_SORT_K || (p.vocab > 2048 * ST_SAMPLE && k <= p.vocab / 16)) {
             // A value that about k tokens or some more reach, from a sample: so much of it that k hardly ever fail to be among those it stands for.
             int every = 1;
@@ -830,18 +941,22 @@ __global__ void __launch_bounds__(ST_THREADS) ns_sample_tokens_kernel(const Samp
             floor = __uint_as_float(__float_as_uint(floor) & 0xFFFF0000u);
             few = true;
         }
-        if (k <= ST_SORT_K) {
+        if (few && k <= ST_WIDE_K) {
             int count = 0;
-            count = me.gather(list_few);
-            if (count >= k) {
+            count = me.template gather<ST_WIDE>([&](auto list) { me.above(me.run_begin(tid), 1, me.run_begin(tid + 1), floor, list); });
+            const bool room = p.each * sizeof(T) >= sizeof(SampleNarrow), wide = count > (room ? ST_LIST / 2 : ST_LIST);
+            if (count >= k && (room || !wide)) {
                 const SampleCuts cuts{k, top_p, p.u[row], least};
                 auto listed = cl.barrier_arrive();         // the first CTA has the others' lists
-                if (rank == 0) st_draw(s, count, cuts, weight, row, p);
+                if (rank == 0) {
+                    if (wide) st_draw_wide(s, *reinterpret_cast<SampleNarrow*>(st_smem + sizeof(SampleShared)), count, cuts, weight, row, p);
+                    else st_draw(s, count, cuts, weight, row, p);
+                }
                 cl.barrier_wait(static_cast<decltype(listed)&&>(listed));
                 return;
             }
             cl.sync();
-            few = count < 0;               // too many, or not enough
+            few = count < 0 || count >= k;                 // too many, or not enough
         }
         auto number = [&](uint64_t) { return (uint64_t)k; };
         cut = me.select(false, few, floor, least, sum, number);

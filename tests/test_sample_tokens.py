@@ -135,6 +135,30 @@ def test_large_tokens_at_regular_places(dev, vocab, dtype):
 
 
 @pytest.mark.gpu
+@pytest.mark.parametrize("dtype", [N.NS_F32, N.NS_BF16])
+@pytest.mark.parametrize("vocab,equal", [(16400, 600), (30000, 1200), (131001, 1900), (40000, 2500)])
+def test_more_equal_candidates_than_are_sorted(dev, vocab, equal, dtype):
+    """Many tokens of one value, or of two, around the cutoffs."""
+    rng = np.random.default_rng(equal)
+    ks = [100, 128, 300, 512, 513, 900, 1024, 1025]
+    rows = 2 * len(ks)
+    x = np.full((rows, vocab), -6.0, np.float32) + rng.random((rows, vocab)).astype(np.float32)
+    for r in range(rows):
+        where = rng.permutation(vocab)[:equal]
+        x[r, where] = 2.0
+        if r >= len(ks):
+            x[r, where[:equal // 3]] = 2.015625
+            x[r, where[:7]] = 3.0 + rng.random(7).astype(np.float32)
+    bits, rounded = bf16(x)
+    x = rounded if dtype == N.NS_BF16 else x
+    for top_p, least in ((1.0, 0.0), (0.5, 0.0), (0.9, 0.3)):
+        s = dict(temperature=np.full(rows, 0.8, np.float32), top_k=np.tile(np.array(ks, np.int32), 2), top_p=np.full(rows, top_p, np.float32), min_p=np.full(rows, least, np.float32),
+                 u=rng.random(rows).astype(np.float32))
+        ids, probs = sample(dev, bits if dtype == N.NS_BF16 else x, dtype, rows, vocab, vocab, s)
+        check(ids, probs, x, s)
+
+
+@pytest.mark.gpu
 def test_temperatures_and_logits_of_every_size(dev):
     rng = np.random.default_rng(7)
     vocab = 20000
