@@ -289,7 +289,7 @@ def test_pages_outside_the_pool(dev, dim, page, batch, prefix):
 
 
 @pytest.mark.gpu
-@pytest.mark.parametrize("dim,group,batch,prefix", [(128, 4, 40, 900), (64, 1, 3, 900), (128, 4, 40, 6000), (64, 4, 100, 4100)])
+@pytest.mark.parametrize("dim,group,batch,prefix", [(128, 4, 40, 900), (64, 1, 3, 900), (128, 4, 40, 6000), (64, 4, 100, 4100), (128, 4, 40, 11000), (64, 4, 100, 8600), (32, 8, 100, 9000)])
 def test_values_alike(dev, dim, group, batch, prefix):
     """Weights add up to one: values that are all alike come back within the rounding of the weights and of the output."""
     s = Setup(dev, dim, 1, group, 64, batch, 1, prefix, [70] * batch)
@@ -301,7 +301,7 @@ def test_values_alike(dev, dim, group, batch, prefix):
 
 
 @pytest.mark.gpu
-@pytest.mark.parametrize("batch,prefix", [(2, 200), (40, 200), (20, 1300)])
+@pytest.mark.parametrize("batch,prefix", [(2, 200), (40, 200), (20, 1300), (40, 1400)])
 def test_a_pool_of_more_than_2_31_elements(dev, batch, prefix):
     dim, kv, page = 128, 8, 64
     n = 2 ** 31 // (kv * page * dim) + 200
@@ -322,10 +322,16 @@ def test_a_pool_of_more_than_2_31_elements(dev, batch, prefix):
 
 
 @pytest.mark.gpu
-def test_replays_with_other_lengths(dev):
+@pytest.mark.parametrize("longer", [False, True])
+def test_replays_with_other_lengths(dev, longer):
     """A recorded call follows the device's positions, length and tables; two recorded calls share the scratch block in stream order."""
     sets = [Setup(dev, 128, 2, 4, 64, 6, 1, 500, [90] * 6, seed=1), Setup(dev, 64, 2, 4, 16, 40, 1, 300, [50] * 40, seed=2), Setup(dev, 128, 2, 4, 16, 48, 1, 2200, [50] * 48, seed=3),
             Setup(dev, 64, 1, 8, 64, 70, 1, 3000, [80] * 70, seed=4)]
+    if longer:                                       # long enough for the tensor-core kernel, between two that are not
+        for s in sets[2:]:
+            s.close()
+        sets[1:] = [Setup(dev, 128, 2, 4, 16, 48, 1, 4700, [50] * 48, seed=3), Setup(dev, 64, 1, 8, 64, 70, 1, 6300, [80] * 70, seed=4), Setup(dev, 128, 2, 2, 64, 40, 1, 5700, [30] * 40, seed=5),
+                    Setup(dev, 32, 2, 8, 32, 70, 1, 6300, [80] * 70, seed=6), sets[1]]
     graphs = []
     for s in sets:
         s.upload()
@@ -360,6 +366,11 @@ def test_runs_repeat_bit_for_bit(dev):
         for _ in range(3):
             assert np.array_equal(s.call(), first)
         s.close()
+    s = Setup(dev, 128, 4, 4, 32, 32, 1, 3600, [200, 3] * 16)
+    s.upload()
+    first = s.call()
+    assert all(np.array_equal(s.call(), first) for _ in range(3))
+    s.close()
 
 
 def test_refusals():

@@ -159,6 +159,22 @@ def test_more_equal_candidates_than_are_sorted(dev, vocab, equal, dtype):
 
 
 @pytest.mark.gpu
+@pytest.mark.parametrize("vocab,dtype", [(380000, N.NS_F32), (760000, N.NS_BF16), (262144, N.NS_F32), (524289, N.NS_BF16)])
+def test_the_largest_vocabularies(dev, vocab, dtype):
+    rng = np.random.default_rng(vocab)
+    rows = 12
+    x = (rng.standard_normal((rows, vocab)) * 2).astype(np.float32)
+    x[:, rng.integers(0, vocab, 30)] += 8
+    x[rows // 2:] *= 0.25
+    bits, rounded = bf16(x)
+    x = rounded if dtype == N.NS_BF16 else x
+    s = dict(temperature=np.tile(np.array([1.0, 0.7, 1.3], np.float32), 4), top_k=np.tile(np.array([0, 50, 1000, 40000], np.int32), 3), top_p=np.tile(np.array([0.9, 1.0], np.float32), 6),
+             min_p=np.zeros(rows, np.float32), u=rng.random(rows).astype(np.float32))
+    ids, probs = sample(dev, bits if dtype == N.NS_BF16 else x, dtype, rows, vocab, vocab, s)
+    check(ids, probs, x, s)
+
+
+@pytest.mark.gpu
 def test_temperatures_and_logits_of_every_size(dev):
     rng = np.random.default_rng(7)
     vocab = 20000

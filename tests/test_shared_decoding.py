@@ -145,6 +145,42 @@ def test_continuations_of_one_prompt(dev, batch, prompt, dim, group, page):
 
 
 @pytest.mark.gpu
+def test_two_device_objects_at_once(dev):
+    """Steps queued on two streams of one GPU, not waited for in between, leave what each leaves alone."""
+    from nn_b200.device import Device
+
+    other = Device(0)
+    steps = 12
+    shapes = [dict(batch=40, prompt=5500, dim=128, group=4, page=64), dict(batch=28, prompt=8000, dim=64, group=8, page=128)]
+    want = []
+    for turn_ in range(2):
+        both = [Step(d, c["batch"], c["prompt"], steps, dim=c["dim"], group=c["group"], page=c["page"], seed=3 + i) for i, (d, c) in enumerate(zip((dev, other), shapes))]
+        for s in both:
+            s.read_prompt()
+            s.us = [s.dev.from_numpy(s.u[t]) for t in range(steps)]
+            s.at = [s.dev.from_numpy(np.full(s.batch, t, np.int32)) for t in range(steps)]
+            s.dev.synchronize()
+        if turn_ == 0:
+            order = [(s, t) for s in both for t in range(steps)]
+        else:
+            order = [(s, t) for t in range(steps) for s in both]
+        for s, t in order:
+            s.d["u"], s.d["pos"] = s.us[t], s.at[t]
+            s.queue()
+            if turn_ == 0:
+                s.dev.synchronize()
+        for s in both:
+            s.dev.synchronize()
+        got = [(s.d["ids"].download(), s.probs.download(), s.o.download((s.batch, s.heads * s.dim))) for s in both]
+        if turn_ == 0:
+            want = got
+        else:
+            assert all(np.array_equal(a, b) for g, w in zip(got, want) for a, b in zip(g, w))
+        for s in both:
+            s.close()
+
+
+@pytest.mark.gpu
 def test_many_draws_from_one_row(dev):
     """A row pitch of 0: every draw of the first token reads the same logits."""
     rng = np.random.default_rng(4)
