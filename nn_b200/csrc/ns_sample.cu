@@ -820,6 +820,8 @@ __global__ void __launch_bounds__(ST_THREADS) ns_sample_tokens_kernel(const Samp
     ns_pdl_wait();
     ns_pdl_trigger();
     cg::cluster_group cl = cg::this_cluster();
+    // (answered before the first write to another CTA's shared memory, which exists only from that CTA's start on; the row is read in between)
+    auto begun = cl.barrier_arrive();
     const int rank = (int)cl.block_rank(), ranks = (int)cl.num_blocks();
     const int row = blockIdx.x / ranks, tid = threadIdx.x;
     const int first = min(rank * p.each, p.vocab), n = min(p.each, p.vocab - first);
@@ -872,6 +874,7 @@ __global__ void __launch_bounds__(ST_THREADS) ns_sample_tokens_kernel(const Samp
     for (int o = 16; o > 0; o >>= 1) best = fmaxf(best, __shfl_xor_sync(0xffffffffu, best, o));
     if ((tid & 31) == 0) s.red[tid >> 5] = best;
     __syncthreads();
+    cl.barrier_wait(static_cast<decltype(begun)&&>(begun));      // every CTA of the cluster runs
     if (tid < ranks) {
         for (int w = 0; w < ST_THREADS / 32; w++) best = fmaxf(best, s.red[w]);
         cl.map_shared_rank(&s, tid)->max[rank] = best;

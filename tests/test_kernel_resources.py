@@ -88,3 +88,23 @@ def test_a_row_ahead_fits_the_longest_rows(report):
     """16384 columns take 1024 threads: 64 registers each."""
     (regs, spill), = [v for n, v in report.items() if "ns_quantize_rows_reg_kernelILi2ELb1ELb1E" in n]
     assert regs <= 64 and spill == 0
+
+
+def _kernels():
+    """(name, body) of every kernel of the sources, comments taken out."""
+    for path in sorted(glob.glob(os.path.join(build.CSRC, "*.cu"))):
+        text = re.sub(r"//[^\n]*", "", open(path).read())
+        for m in re.finditer(r"__global__[^;{]*?\b(\w+_kernel)\([^;{]*?\)\s*\{(.*?)\n\}", text, re.S):
+            yield m.groups()
+
+
+def test_a_cluster_has_begun_before_another_ctas_shared_memory_is_touched():
+    """Shared memory of a cluster's other CTAs exists from their start to their end: a kernel that reads or writes it has waited for a barrier of the cluster first."""
+    seen = set()
+    for name, body in _kernels():
+        remote = re.search(r"map_shared_rank\(|ns_mapa\(", body)
+        if remote is None:
+            continue
+        seen.add(name)
+        assert re.search(r"\bcl\.sync\(\)|\bcl\.barrier_wait\(|ns_cluster_sync\(\)", body[:remote.start()]), name
+    assert "ns_sample_tokens_kernel" in seen
