@@ -108,3 +108,49 @@ def test_a_cluster_has_begun_before_another_ctas_shared_memory_is_touched():
         seen.add(name)
         assert re.search(r"\bcl\.sync\(\)|\bcl\.barrier_wait\(|ns_cluster_sync\(\)", body[:remote.start()]), name
     assert "ns_sample_tokens_kernel" in seen
+
+
+# registers and bytes loaded back from spills that any build may have
+@pytest.mark.parametrize("kernel,most_registers,most_spilled", [
+    ("ns_rotary_kernel", 64, 48), ("ns_kv_append_rotary_kernelILb[01]ELi\\dELin1E", 64, 36), ("ns_kv_append_rotary_kernelILb[01]ELi\\dELi1E", 80, 164),
+    # three CTAs of 128 threads an SM; the launch's registers that setmaxnreg deals out (the most it can hold); two CTAs of 512
+    ("ns_attention_shared_walk_kernel", 168, 0), ("ns_attention_shared_fold_kernel", 80, 0), ("ns_attention_shared_tile_kernel", 168, 568), ("ns_sample_tokens_kernel", 64, 136),
+])
+def test_kernels_of_a_shared_prompt_keep_their_registers(report, kernel, most_registers, most_spilled):
+    builds = {n: v for n, v in report.items() if re.search(r"\d" + kernel, n)}
+    assert builds
+    assert all(regs <= most_registers and spill <= most_spilled for regs, spill in builds.values()), builds
+
+
+def test_every_programmatic_launch_is_known():
+    """ns_launch_pdl is given a kernel by its name or by a variable of the function around it.  Of attention over a shared prefix, the kernel that joins waits
+    before it reads anything, and the kernel that walks where it runs alone; beside the tensor-core kernel it may go without for the reason given here."""
+    bodies, launched = {}, set()
+    for name, body in _kernels():
+        bodies[name] = body
+    for path in sorted(glob.glob(os.path.join(build.CSRC, "*.cu"))):
+        text = re.sub(r"//[^\n]*", "", open(path).read())
+        for call in re.finditer(r"ns_launch_pdl\(\s*(\w+)", text):
+            if call.group(1) in bodies:
+                launched.add(call.group(1))
+                continue
+            # the nearest definition before the call, of which a ?: names two, or a lambda's parameter and what it is called with
+            before = text[:call.start()]
+            found = list(re.finditer(r"auto %s = ([^;]*);" % call.group(1), before))
+            names = re.findall(r"\b(ns_\w+_kernel)", found[-1].group(1)) if found else []
+            if not names:
+                names = re.findall(r"launch\((ns_\w+_kernel)", text)
+            assert names, (path, text[call.start():call.start() + 80])
+            launched |= set(names)
+    assert {"ns_attention_shared_walk_kernel", "ns_attention_shared_fold_kernel"} <= launched
+    fold = bodies["ns_attention_shared_fold_kernel"]
+    assert not re.search(r"\bp\.", fold[:fold.index("ns_pdl_wait()")])
+    # Walking beside the tensor-core kernel, the first wait is left out: that kernel is launched plainly, so that all before it has completed, and nothing of its own is read.  Its last
+    # CTA waits for it, since the kernel that joins both follows this one alone.
+    walk = bodies["ns_attention_shared_walk_kernel"]
+    start, end = walk.index("ns_pdl_wait()"), walk.rindex("ns_pdl_wait()")
+    assert start < end and re.search(r"if \(p\.beside == nullptr\) \{\s*$", walk[:start]) and re.search(r"if \(last != 0\) \{[^}]*$", walk[:end])
+    tiles = open(os.path.join(build.CSRC, "ns_attention_shared_tc.cu")).read()
+    assert re.search(r"kernel<<<[^>]*d->stream>>>\(maps, p\);", tiles) and "ns_launch_pdl" not in tiles
+    tile = bodies["ns_attention_shared_tile_kernel"]
+    assert tile.index("ns_pdl_wait()") < tile.index("ns_pdl_trigger()") < tile.index("p.s.prefix_len")
