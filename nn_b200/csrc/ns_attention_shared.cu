@@ -4,8 +4,8 @@
 //
 // Softmax over a union of key sets is a fold: every part gives (maximum m, sum l of e^(s - m), weighted values o relative to m), and parts fold as
 //   M = max m,  L = sum l e^(m - M),  O = sum o e^(m - M);  the result is O / L.
-// So the prefix is one part (or several, by position) for the rows of ALL sequences together, whose keys and values are then read once and not once for each
-// sequence, and each sequence's own pages are another.  Every part is computed from its keys alone, and parts fold in a fixed order.
+// So the prefix is one part (or several, by position) for the rows of ALL sequences together, whose keys and values are then read once for every tile of rows (256 of the
+// tensor-core kernel, 8 or 16 here) and not once for each sequence, and each sequence's own pages are another.  Every part is computed from its keys alone, and parts fold in a fixed order.
 //
 // Rows: the query heads of a key/value head share its cached rows; row r of a key/value head is token r / group (sequence * steps + i), query head
 // r % group of its group.

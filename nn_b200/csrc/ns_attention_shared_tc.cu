@@ -163,6 +163,9 @@ __device__ __forceinline__ uint64_t st_fma2(uint64_t a, uint64_t b, uint64_t c)
     return y;
 }
 // P = 2^(s scale + neg_m) of pairs [C0, C1) of the 64 scores from FIRST on, as bf16; the sums of P before that rounding go onto `sum`.
+// The MMA takes P in 16 bits: each weight is off by half a step, 2^-8 of itself at most, to either side, which over many keys adds little to the rounding of the output (0.0020 to 0.0025
+// of its rms in all for 0.0017).  A second half of every weight, as the walking kernel has it, would be some three instructions more to the
+// four that each score takes here, which bound this kernel.
 template <int FIRST, int C0, int C1>
 __device__ __forceinline__ void st_exponentials(const float (&s)[ST_KB], float scale, float neg_m, uint64_t (&sum)[2], uint32_t (&pk)[32])
 {
@@ -646,6 +649,7 @@ bool ns_attention_shared_tiles_fit(const NsDevice* d, const SharedParams& s, int
     // line, us, this kernel's way and the other's (rows of a key/value head x heads x keys x columns): 128 x 2 x 3333 x 128 22.6, 15.8; 64 x 8 x 2000 x 128 17.5, 17.2; 64 x 16 x 2500 x 64 21.0,
     // 18.3; 256 x 4 x 1600 x 128 24.8, 20.7; 256 x 8 x 700 x 128 20.0, 23.0; 256 x 2 x 4000 x 128 21.6, 23.2; 128 x 8 x 2500 x 128 27.2, 32.3; 64 x 16 x 5000 x 64 24.6, 27.9; 24 x 8 x 16000 x 128
     // 31.8, 33.6; 20 x 32 x 4000 x 128 42.0, 36.4; 20 x 16 x 16000 x 128 45.7, 54.8; 16 x 32 x 16000 x 128 67.6, 62.8; 8 x 8 x 64000 x 128 64.0, 51.3.
+    // (One product for all leaves 256 x 8 x 700, 1 430 000, on the slower side: more rows pay earlier than fewer, 64 x 16 x 2500 x 64 at nearly the same product the other way round.)
     const int64_t rows = (int64_t)s.batch * s.steps * s.group;
     const double work = (double)rows * s.kv_heads * ((double)s.prefix_pages * (1 << s.page_shift)) * head_dim;
     if (rows <= 16 || work < (rows >= 24 ? 1.7e6 : 4e6) * 128) return false;

@@ -11,9 +11,9 @@
 // definition's.)
 //
 // A cluster of 1 to 8 CTAs holds a row in shared memory; it is read from global memory once.  What remains costs passes over shared memory:
-//   - A top-k of up to ST_WIDE_K: a histogram of every 8th token over (max - x) / T, 45 bins to each halving of the weight, names a cutoff that hardly ever fails to leave k candidates and
-//     leaves few more; they are gathered into one CTA.  Few are sorted (value, then index), cut by all three rules, sorted by index and drawn from; of more, the three places (of the
-//     k-th token, of p of the weight, of u of what is left) are found by a histogram and the tokens of one bin each.  (64 rows of 32 000 in turn 34.9 us with cutoffs of the whole cluster, so 27.1.)
+//   - A top-k of up to ST_WIDE_K: a histogram of every 8th token (of every one, in vocabularies up to 16384) over (max - x) / T, 45 bins to each halving of the weight, names
+//     a cutoff that hardly ever fails to leave k candidates and leaves few more; they are gathered into one CTA.  Few are sorted (value, then index), cut by all three rules, sorted by index and drawn from; of more, the three places (of the
+//     k-th token, of p of the weight, of u of what is left) are found by a histogram and the tokens of one bin each.  (64 rows of 32 000 in turn 34.9 us with cutoffs of the whole cluster, so 27.7.)
 //   - Else cutoffs are found one after the other: a histogram, by number (from such a cutoff on) or by weight, names the bin in which a cutoff lies, and that bin's tokens
 //     alone are gathered and sorted (or, where they are too many, counted by the bits of x, 11 at a time).  The draw is then one more pass over the row, or, after a
 //     cutoff by weight, the sums of the pass that gathered.
@@ -40,7 +40,6 @@ constexpr int ST_SORT_K = 128;             // a top-k whose candidates are looke
 constexpr int ST_WIDE = 4 * ST_LIST;       // candidates that one CTA cuts with histograms of its own: four a thread
 constexpr int ST_WIDE_K = 1024;            // the largest top-k whose candidates one CTA takes
 constexpr int ST_SAMPLE = 8;               // its cutoff is guessed from every 8th token
-constexpr uint32_t ST_NO_CUT = 0xFFFFFFFFu;
 
 struct SampleArgs {
     const void* x;
@@ -222,8 +221,8 @@ __device__ __forceinline__ uint64_t st_aim(float u, uint64_t total)
 
 // e^(-d / T) in units of 2^-42, d = max - x >= 0, within 2^-33 of itself (64-bit floats would take five times as long here: a warp's instruction 16 cycles).
 // d is a float and the rest of it, exactly; t = d / (T ln 2) the same to 2^-46 of itself; t = n + i / 1024 + r with |r| <= 2^-11;
-// 2^(-i / 1024) from a table, 2^(-r) = 1 + q with q a polynomial of degree 3 and below 2^-12, so that its float's error counts 2^-36; the product is rounded to an
-// integer once, and shifted by n.
+// 2^(-i / 1024) from a table, 2^(-r) = 1 + q with q a polynomial of degree 3 and below 2^-11.5 (0.7 * 2^-11), so that each rounding of its float counts 2^-35.5; its product with
+// the table's 2^42, below 2^31 therefore, is rounded to an integer of 32 bits once, added to the table's and shifted by n.
 __device__ __forceinline__ uint64_t st_pair(float lo, float hi)
 {
     uint64_t y;
